@@ -385,6 +385,100 @@ ms_status ms_generate_long(ms_model* model, const float* audio, int64_t n_sample
                            const ms_streaming_config* config, int32_t* ids_out, int32_t cap,
                            int32_t* n_out, ms_gen_stats* stats);
 
+/* ------------------------------------------------------------------- 4-bit paged K/V cache
+ *
+ * Operators on device memory for callers that hold their own K/V cache (no counterpart in the
+ * reference, whose caches are dense and fp32 or fp16, MoonshineLayers.swift:106-125); the
+ * batched engine runs on them too (page tables always, the cross-attention K/V of
+ * ms_options.cross_kv_bits = 4).  Every pointer below is device memory of `device`
+ * (-1: the current device), every call only enqueues work on `stream` (a cudaStream_t of
+ * that device; null: the legacy default stream) and neither allocates nor synchronises, so
+ * all of them can be captured into a CUDA graph; a graph replays with the lengths, tables
+ * and pages that the device memory then holds.  Argument errors are found before anything
+ * is enqueued.
+ *
+ * Pages.  A pool holds `pages` pages of page_size positions (a multiple of 16), each position
+ * with kv_heads K and V vectors of head_dim values (a multiple of 8, at most 128).  A vector's
+ * values are cut into groups of 64 (the last one shorter); a group is stored as 4-bit codes c,
+ * an fp16 scale s and an fp16 bias b (the affine form of the quantized checkpoints) and
+ * stands for s c + b: b = fp16(min), s = fp16(fp32((max - min) / 15)), c = how many of the
+ * borders b + (k + 1/2) s, k = 0 .. 14, are <= the value.  Values beyond +-65504 are
+ * stored as +-65504; a group that holds a NaN reads as NaNs.  A position takes
+ * ms_kv4_position_bytes(head_dim) bytes per head, head h of page p lies at
+ * base + p * page_stride + h * head_stride and takes page_size times that. */
+typedef enum { MS_F32 = 0, MS_F16 = 1, MS_BF16 = 2 } ms_dtype;
+
+typedef struct {
+    void* base;               /* 16-byte aligned */
+    int64_t page_stride;      /* bytes between pages, a multiple of 16 */
+    int64_t head_stride;      /* bytes between the heads of a page, a multiple of 16 */
+    int32_t pages, kv_heads, head_dim, page_size;
+} ms_kv4_pool;
+
+/* Bytes of one position's K and V for one head: head_dim + 8 * ceil(head_dim / 64); 0 for a
+ * head_dim that is not supported. */
+int32_t ms_kv4_position_bytes(int32_t head_dim);
+
+/* Block tables and slot maps from request lengths, on the device.  Row b of `rows` holds
+ * lengths[b] positions in the first ceil(lengths[b] / page_size) pages of its table row and
+ * appends new_tokens[b] more (negative entries count as 0; their sum, and each row's total,
+ * stay below 2^31).  The pages it lacks are taken in row order from free_pages [n_free]
+ * (null: the pages 0 .. n_free - 1) and entered behind the ones it has; the entries behind
+ * them become -1.  Entries of held pages are left as they are.
+ *   block_table [rows][table_stride]  width entries per row, read and written
+ *   slots       [n_slots] slot (page * page_size + offset) of every new token, row after row;
+ *               -1 where its page is missing (no free page left, held entry negative, table
+ *               too narrow) and behind the last token
+ *   cu_new      [rows + 1] first slot of each row, then the number of new tokens
+ *   counts      [2] pages that the rows need (entries past n_free are -1), new tokens */
+ms_status ms_kv_block_tables(const int32_t* lengths, const int32_t* new_tokens, int32_t rows, int32_t page_size,
+                             const int32_t* free_pages, int32_t n_free, int32_t* block_table, int32_t width,
+                             int64_t table_stride, int64_t* slots, int64_t n_slots, int32_t* cu_new,
+                             int32_t* counts, int32_t device, void* stream);
+
+/* K and V of `tokens` tokens ([tokens][kv_heads][head_dim], strides in elements, the head dim
+ * contiguous) into their slots.  A slot outside the pool (-1) is skipped.  Slots are distinct:
+ * of a slot given twice the position's value is unspecified. */
+ms_status ms_kv4_append(const ms_kv4_pool* pool, const void* k, const void* v, int32_t dtype, int64_t tokens,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                        int64_t v_head_stride, const int64_t* slots, int32_t device, void* stream);
+/* The values that the slots' codes stand for, rounded to dtype (zeros for a slot outside the
+ * pool), as ms_stream_memory reads a stream's memory rows. */
+ms_status ms_kv4_read(const ms_kv4_pool* pool, void* k_out, void* v_out, int32_t dtype, int64_t tokens,
+                      int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                      int64_t v_head_stride, const int64_t* slots, int32_t device, void* stream);
+
+/* Attention of new queries over the pages.  Row b's queries are the tokens cu_q[b] ..
+ * cu_q[b + 1] - 1 of q (cu_q null: token b alone); position t < lens[b] of row b lies in page
+ * block_table[b][t / page_size], and a position whose entry is outside the pool, or past the
+ * table's width, is not there.  With `causal`, query i of n sees only the positions up to
+ * lens[b] - n + i (lens counts the queries' own positions); otherwise all.  Query head h reads
+ * K/V head h / (heads / kv_heads).  out = softmax(scale q k^T) v, zeros for a query that sees
+ * nothing; tokens of no row are left as they are.  Sums and softmax are fp32; the products
+ * take the codes exactly and q and the probabilities in fp16 planes: two of each for MS_F32, two
+ * of the probabilities for MS_F16, one of each for MS_BF16. */
+typedef struct {
+    const void* q;                                /* [q_tokens][heads][head_dim] */
+    void* out;                                    /* the same shape; may not overlap q */
+    int64_t q_tokens;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  /* elements */
+    const int32_t* block_table;                   /* [rows][table_stride], width entries each */
+    int64_t table_stride;
+    const int32_t* lens;                          /* [rows] */
+    const int32_t* cu_q;                          /* nullable, [rows + 1] ascending */
+    int32_t dtype, heads, rows, width;
+    int32_t max_q;                                /* at least every row's queries; those past it are left out */
+    int32_t causal;
+    float scale;                                  /* 0: head_dim^-1/2 */
+    int32_t reserved;
+} ms_kv4_attention_args;
+
+/* Workspace bytes of ms_kv4_attention, by the sizes in its arguments alone (0: none needed).
+ * Calls whose GPU work can overlap (two streams, two graphs) need a workspace each. */
+int64_t ms_kv4_attention_workspace(const ms_kv4_pool* pool, const ms_kv4_attention_args* args);
+ms_status ms_kv4_attention(const ms_kv4_pool* pool, const ms_kv4_attention_args* args, void* workspace,
+                           int64_t workspace_bytes, int32_t device, void* stream);
+
 /* ------------------------------------------------------------------- diagnostics */
 
 /* Thread-local message of the last failing call on this thread ("" if none). */
@@ -405,7 +499,8 @@ ms_status ms_decode_trace(ms_model* model, uint64_t* stamps_out, int32_t cap, in
 /* Library version string. */
 const char* ms_version(void);
 /* sizeof of one of this header's structs by its name ("ms_options", "ms_model_config",
- * "ms_gen_params", "ms_gen_stats", "ms_alignment", "ms_streaming_config"), 0 for any other
+ * "ms_gen_params", "ms_gen_stats", "ms_alignment", "ms_streaming_config", "ms_kv4_pool",
+ * "ms_kv4_attention_args"), 0 for any other
  * name: a binding in another language checks its own layouts against it at load. */
 size_t ms_struct_size(const char* name);
 

@@ -2,6 +2,7 @@
 // every launcher enqueues on `stream` and returns cudaGetLastError().
 #pragma once
 
+#include <algorithm>
 #include <utility>
 
 #include <cuda_runtime.h>
@@ -383,6 +384,46 @@ size_t cross_batch_part_floats(int B, int H, int hd, int max_frames);
 cudaError_t launch_gather_cross(const float* const* src32, const void* const* src16, const int* mcap,
                                 const int* frames, const int* off, int B, int segs, int hd, int m_cap, float* dst32,
                                 void* dst16, cudaStream_t s);
+
+// ---------------------------------------------------------------- 4-bit paged K/V cache
+enum Kv4Type { KV4_F32 = 0, KV4_F16 = 1, KV4_BF16 = 2 };
+// Pages of 4-bit keys and values (layout: kv4.cuh); strides in bytes, multiples of 16.
+struct Kv4Pool {
+    void* base = nullptr;
+    int pages = 0, kv_heads = 0, head_dim = 0, page_size = 0;
+    long long page_stride = 0, head_stride = 0;
+};
+// Row b's queries are tokens cu_q[b] .. cu_q[b + 1] of q (null: token b), at most max_q; they
+// see the first lens[b] positions of the row's pages, query i of n under `causal` only those
+// up to lens[b] - n + i.  Strides in elements, the head dim contiguous.
+struct Kv4Attention {
+    const void* q = nullptr;
+    void* out = nullptr;
+    int dtype = KV4_F32, heads = 0;
+    long long q_tokens = 0;
+    long long q_token_stride = 0, q_head_stride = 0, out_token_stride = 0, out_head_stride = 0;
+    const int* table = nullptr;
+    long long table_stride = 0;
+    int rows = 0, width = 0;
+    const int* lens = nullptr;
+    const int* cu_q = nullptr;
+    int max_q = 1, causal = 0;
+    float scale = 1.f;
+};
+cudaError_t launch_block_tables(const int* lengths, const int* added, int rows, int page, const int* free_pages,
+                                int n_free, int* table, int width, long long table_stride, long long* slots,
+                                long long n_slots, int* cu, int* counts, cudaStream_t s);
+// k, v [tokens][kv_heads][head_dim] (strides in elements) to / from slots page * page_size +
+// offset; a slot outside the pool is skipped by append and reads as zeros.
+cudaError_t launch_kv4_append(const Kv4Pool& pool, const void* k, const void* v, int dtype, long long tokens,
+                              long long k_token_stride, long long k_head_stride, long long v_token_stride,
+                              long long v_head_stride, const long long* slots, cudaStream_t s);
+cudaError_t launch_kv4_read(const Kv4Pool& pool, void* k, void* v, int dtype, long long tokens,
+                            long long k_token_stride, long long k_head_stride, long long v_token_stride,
+                            long long v_head_stride, const long long* slots, cudaStream_t s);
+// Workspace bytes of launch_kv4_attention (by sizes alone, not by the lengths on the device).
+size_t kv4_attention_workspace(const Kv4Pool& pool, const Kv4Attention& a);
+cudaError_t launch_kv4_attention(const Kv4Pool& pool, const Kv4Attention& a, void* workspace, cudaStream_t s);
 
 // Head-clustered batch-1 decode (one 8-CTA cluster per head, packed per-CTA weight streams).
 struct ClusterGeom {

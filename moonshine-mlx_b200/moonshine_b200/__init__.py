@@ -25,6 +25,8 @@ from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
 
+from . import kv4 as _kv4
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmoonshine_b200.so")
 
@@ -154,6 +156,7 @@ def _load_lib() -> C.CDLL:
         "ms_version": (C.c_char_p, []),
         "ms_struct_size": (C.c_size_t, [C.c_char_p]),
     }
+    sigs.update(_kv4.SIGNATURES)
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -161,7 +164,7 @@ def _load_lib() -> C.CDLL:
     # the structs passed by pointer must have the library's layout
     for cname, cls in (("ms_options", _Options), ("ms_model_config", _ModelConfig), ("ms_gen_params", _GenParams),
                        ("ms_gen_stats", _GenStats), ("ms_alignment", _Alignment),
-                       ("ms_streaming_config", _StreamingConfig)):
+                       ("ms_streaming_config", _StreamingConfig)) + _kv4.STRUCTS:
         if lib.ms_struct_size(cname.encode()) != C.sizeof(cls):
             raise ImportError(f"{cname}: {C.sizeof(cls)} bytes here, {lib.ms_struct_size(cname.encode())} in "
                               f"{LIB_PATH} (a library built from another header)")
@@ -728,6 +731,10 @@ class MoonshineModel:
             else:
                 cur.append(t)
         return segs
+
+
+# 4-bit paged K/V cache operators on torch CUDA tensors
+from .kv4 import kv4_append, kv4_attention, kv4_pool, kv4_position_bytes, kv4_read, kv_block_tables  # noqa: E402,F401
 
 
 def kernel_launches() -> int:
