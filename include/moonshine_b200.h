@@ -424,29 +424,38 @@ int32_t ms_kv4_position_bytes(int32_t head_dim);
  * appends new_tokens[b] more (negative entries count as 0; their sum, and each row's total,
  * stay below 2^31).  The pages it lacks are taken in row order from free_pages [n_free]
  * (null: the pages 0 .. n_free - 1) and entered behind the ones it has; the entries behind
- * them become -1.  Entries of held pages are left as they are.
- *   block_table [rows][table_stride]  width entries per row, read and written
- *   slots       [n_slots] slot (page * page_size + offset) of every new token, row after row;
- *               -1 where its page is missing (no free page left, held entry negative, table
- *               too narrow) and behind the last token
- *   cu_new      [rows + 1] first slot of each row, then the number of new tokens
- *   counts      [2] pages that the rows need (entries past n_free are -1), new tokens */
-ms_status ms_kv_block_tables(const int32_t* lengths, const int32_t* new_tokens, int32_t rows, int32_t page_size,
-                             const int32_t* free_pages, int32_t n_free, int32_t* block_table, int32_t width,
-                             int64_t table_stride, int64_t* slots, int64_t n_slots, int32_t* cu_new,
-                             int32_t* counts, int32_t device, void* stream);
+ * them become -1.  Entries of held pages are left as they are. */
+typedef struct {
+    const int32_t* lengths;       /* [rows] */
+    const int32_t* new_tokens;    /* [rows] */
+    const int32_t* free_pages;    /* nullable [n_free] */
+    int32_t* block_table;         /* [rows][table_stride], width entries per row; read and written */
+    int64_t* slots;               /* out [n_slots]: slot (page * page_size + offset) of every new token,
+                                     row after row; -1 where its page is missing (no free page left,
+                                     held entry negative, table too narrow) and behind the last token */
+    int32_t* cu_new;              /* out [rows + 1]: first slot of each row, then the number of new tokens */
+    int32_t* counts;              /* out [2]: pages that the rows need (those past n_free are -1), new tokens */
+    int64_t table_stride, n_slots;
+    int32_t rows, width, page_size, n_free;
+} ms_kv_tables;
+ms_status ms_kv_block_tables(const ms_kv_tables* args, int32_t device, void* stream);
 
-/* K and V of `tokens` tokens ([tokens][kv_heads][head_dim], strides in elements, the head dim
- * contiguous) into their slots.  A slot outside the pool (-1) is skipped.  Slots are distinct:
+/* K and V of `tokens` tokens, [tokens][kv_heads][head_dim] (strides in elements, the head dim
+ * contiguous), and their slots. */
+typedef struct {
+    void* k;                      /* read by ms_kv4_append, written by ms_kv4_read */
+    void* v;
+    const int64_t* slots;         /* [tokens] */
+    int64_t tokens;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int32_t dtype, reserved;      /* ms_dtype */
+} ms_kv4_tokens;
+/* The tokens into their slots.  A slot outside the pool (-1) is skipped.  Slots are distinct:
  * of a slot given twice the position's value is unspecified. */
-ms_status ms_kv4_append(const ms_kv4_pool* pool, const void* k, const void* v, int32_t dtype, int64_t tokens,
-                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                        int64_t v_head_stride, const int64_t* slots, int32_t device, void* stream);
+ms_status ms_kv4_append(const ms_kv4_pool* pool, const ms_kv4_tokens* tokens, int32_t device, void* stream);
 /* The values that the slots' codes stand for, rounded to dtype (zeros for a slot outside the
  * pool), as ms_stream_memory reads a stream's memory rows. */
-ms_status ms_kv4_read(const ms_kv4_pool* pool, void* k_out, void* v_out, int32_t dtype, int64_t tokens,
-                      int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                      int64_t v_head_stride, const int64_t* slots, int32_t device, void* stream);
+ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* tokens, int32_t device, void* stream);
 
 /* Attention of new queries over the pages.  Row b's queries are the tokens cu_q[b] ..
  * cu_q[b + 1] - 1 of q (cu_q null: token b alone); position t < lens[b] of row b lies in page
@@ -454,9 +463,9 @@ ms_status ms_kv4_read(const ms_kv4_pool* pool, void* k_out, void* v_out, int32_t
  * table's width, is not there.  With `causal`, query i of n sees only the positions up to
  * lens[b] - n + i (lens counts the queries' own positions); otherwise all.  Query head h reads
  * K/V head h / (heads / kv_heads).  out = softmax(scale q k^T) v, zeros for a query that sees
- * nothing; tokens of no row are left as they are.  Sums and softmax are fp32; the products
- * take the codes exactly and q and the probabilities in fp16 planes: two of each for MS_F32, two
- * of the probabilities for MS_F16, one of each for MS_BF16. */
+ * nothing; tokens of no row are left as they are.  Softmax and sums are fp32; the products take
+ * the codes exactly, q as fixed point of 16 bits (MS_F32: 24) relative to each (token, head)'s
+ * largest value, and the probabilities as one fp16 value (MS_BF16) or two. */
 typedef struct {
     const void* q;                                /* [q_tokens][heads][head_dim] */
     void* out;                                    /* the same shape; may not overlap q */
@@ -499,8 +508,8 @@ ms_status ms_decode_trace(ms_model* model, uint64_t* stamps_out, int32_t cap, in
 /* Library version string. */
 const char* ms_version(void);
 /* sizeof of one of this header's structs by its name ("ms_options", "ms_model_config",
- * "ms_gen_params", "ms_gen_stats", "ms_alignment", "ms_streaming_config", "ms_kv4_pool",
- * "ms_kv4_attention_args"), 0 for any other
+ * "ms_gen_params", "ms_gen_stats", "ms_alignment", "ms_streaming_config", "ms_kv_tables",
+ * "ms_kv4_pool", "ms_kv4_tokens", "ms_kv4_attention_args"), 0 for any other
  * name: a binding in another language checks its own layouts against it at load. */
 size_t ms_struct_size(const char* name);
 

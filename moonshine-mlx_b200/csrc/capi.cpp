@@ -187,7 +187,9 @@ size_t ms_struct_size(const char* name) {
     if (n == "ms_gen_stats") return sizeof(ms_gen_stats);
     if (n == "ms_alignment") return sizeof(ms_alignment);
     if (n == "ms_streaming_config") return sizeof(ms_streaming_config);
+    if (n == "ms_kv_tables") return sizeof(ms_kv_tables);
     if (n == "ms_kv4_pool") return sizeof(ms_kv4_pool);
+    if (n == "ms_kv4_tokens") return sizeof(ms_kv4_tokens);
     if (n == "ms_kv4_attention_args") return sizeof(ms_kv4_attention_args);
     return 0;
 }

@@ -53,6 +53,17 @@ int elem_size(int32_t dtype) {
     return dtype == MS_F32 ? 4 : 2;
 }
 
+int type_of(int32_t dtype) { return dtype == MS_F32 ? KV4_F32 : dtype == MS_F16 ? KV4_F16 : KV4_BF16; }
+
+void check_tokens(const ms_kv4_tokens* t) {
+    need(t != nullptr, "null tokens");
+    const int es = elem_size(t->dtype);
+    need(t->tokens >= 0, "tokens must not be negative");
+    if (t->tokens == 0) return;
+    need(t->k && t->v && t->slots, "null k, v or slots");
+    need(aligned(t->k, es) && aligned(t->v, es), "k and v must be aligned to their type");
+}
+
 void check_head_dim(int32_t hd) {
     if (ms_kv4_position_bytes(hd) == 0)
         throw MsError(MS_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 from 8 to 128, not " + std::to_string(hd));
@@ -98,7 +109,7 @@ Kv4Attention attention_of(const ms_kv4_pool* pool, const ms_kv4_attention_args* 
     Kv4Attention k;
     k.q = a->q;
     k.out = a->out;
-    k.dtype = a->dtype == MS_F32 ? KV4_F32 : a->dtype == MS_F16 ? KV4_F16 : KV4_BF16;
+    k.dtype = type_of(a->dtype);
     k.heads = a->heads;
     k.q_tokens = a->q_tokens;
     k.q_token_stride = a->q_token_stride;
@@ -129,56 +140,45 @@ int32_t ms_kv4_position_bytes(int32_t head_dim) {
     return head_dim + 8 * ((head_dim + 63) / 64);
 }
 
-ms_status ms_kv_block_tables(const int32_t* lengths, const int32_t* new_tokens, int32_t rows, int32_t page_size,
-                             const int32_t* free_pages, int32_t n_free, int32_t* block_table, int32_t width,
-                             int64_t table_stride, int64_t* slots, int64_t n_slots, int32_t* cu_new,
-                             int32_t* counts, int32_t device, void* stream) {
+ms_status ms_kv_block_tables(const ms_kv_tables* t, int32_t device, void* stream) {
     return checked([&] {
-        need(rows >= 0 && width >= 0 && n_free >= 0, "sizes must not be negative");
-        need(n_slots >= 0 && n_slots < (int64_t)1 << 31, "n_slots must be from 0 to 2^31 - 1");
-        need(page_size > 0, "page_size must be positive");
-        need(cu_new && counts, "null cu_new or counts");
-        need(rows == 0 || (lengths && new_tokens), "null lengths or new_tokens");
-        need(rows == 0 || width == 0 || block_table, "null block_table");
-        need(rows <= 1 || table_stride >= width, "table_stride is smaller than width");
-        need(n_slots == 0 || slots, "null slots");
+        need(t != nullptr, "null arguments");
+        need(t->rows >= 0 && t->width >= 0 && t->n_free >= 0, "sizes must not be negative");
+        need(t->n_slots >= 0 && t->n_slots < (int64_t)1 << 31, "n_slots must be from 0 to 2^31 - 1");
+        need(t->page_size > 0, "page_size must be positive");
+        need(t->cu_new && t->counts, "null cu_new or counts");
+        need(t->rows == 0 || (t->lengths && t->new_tokens), "null lengths or new_tokens");
+        need(t->rows == 0 || t->width == 0 || t->block_table, "null block_table");
+        need(t->rows <= 1 || t->table_stride >= t->width, "table_stride is smaller than width");
+        need(t->n_slots == 0 || t->slots, "null slots");
         DeviceScope d(device);
-        MSB_CUDA(launch_block_tables(lengths, new_tokens, rows, page_size, free_pages, n_free, block_table, width,
-                                     table_stride, reinterpret_cast<long long*>(slots), n_slots, cu_new, counts,
+        MSB_CUDA(launch_block_tables(t->lengths, t->new_tokens, t->rows, t->page_size, t->free_pages, t->n_free,
+                                     t->block_table, t->width, t->table_stride,
+                                     reinterpret_cast<long long*>(t->slots), t->n_slots, t->cu_new, t->counts,
                                      reinterpret_cast<cudaStream_t>(stream)));
     });
 }
 
-ms_status ms_kv4_append(const ms_kv4_pool* pool, const void* k, const void* v, int32_t dtype, int64_t tokens,
-                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                        int64_t v_head_stride, const int64_t* slots, int32_t device, void* stream) {
+ms_status ms_kv4_append(const ms_kv4_pool* pool, const ms_kv4_tokens* t, int32_t device, void* stream) {
     return checked([&] {
         const Kv4Pool p = pool_of(pool);
-        const int es = elem_size(dtype);
-        need(tokens >= 0, "tokens must not be negative");
-        if (tokens == 0 || p.pages == 0) return;
-        need(k && v && slots, "null k, v or slots");
-        need(aligned(k, es) && aligned(v, es), "k and v must be aligned to their type");
+        check_tokens(t);
+        if (t->tokens == 0 || p.pages == 0) return;
         DeviceScope d(device);
-        MSB_CUDA(launch_kv4_append(p, k, v, dtype, tokens, k_token_stride, k_head_stride, v_token_stride,
-                                   v_head_stride, reinterpret_cast<const long long*>(slots),
+        MSB_CUDA(launch_kv4_append(p, t->k, t->v, type_of(t->dtype), t->tokens, t->k_token_stride, t->k_head_stride,
+                                   t->v_token_stride, t->v_head_stride, reinterpret_cast<const long long*>(t->slots),
                                    reinterpret_cast<cudaStream_t>(stream)));
     });
 }
 
-ms_status ms_kv4_read(const ms_kv4_pool* pool, void* k_out, void* v_out, int32_t dtype, int64_t tokens,
-                      int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                      int64_t v_head_stride, const int64_t* slots, int32_t device, void* stream) {
+ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* t, int32_t device, void* stream) {
     return checked([&] {
         const Kv4Pool p = pool_of(pool);
-        const int es = elem_size(dtype);
-        need(tokens >= 0, "tokens must not be negative");
-        if (tokens == 0) return;
-        need(k_out && v_out && slots, "null k_out, v_out or slots");
-        need(aligned(k_out, es) && aligned(v_out, es), "k_out and v_out must be aligned to their type");
+        check_tokens(t);
+        if (t->tokens == 0) return;
         DeviceScope d(device);
-        MSB_CUDA(launch_kv4_read(p, k_out, v_out, dtype, tokens, k_token_stride, k_head_stride, v_token_stride,
-                                 v_head_stride, reinterpret_cast<const long long*>(slots),
+        MSB_CUDA(launch_kv4_read(p, t->k, t->v, type_of(t->dtype), t->tokens, t->k_token_stride, t->k_head_stride,
+                                 t->v_token_stride, t->v_head_stride, reinterpret_cast<const long long*>(t->slots),
                                  reinterpret_cast<cudaStream_t>(stream)));
     });
 }

@@ -7,7 +7,7 @@ torch = pytest.importorskip("torch")
 
 import kv4_reference as ref  # noqa: E402
 import moonshine_b200 as mb  # noqa: E402
-from moonshine_b200.kv4 import _Kv4AttentionArgs, _Kv4Pool  # noqa: E402
+from moonshine_b200 import kv4  # noqa: E402
 
 INVALID, CAPACITY, UNSUPPORTED = 1, 9, 8
 
@@ -43,7 +43,14 @@ def test_reference_quantizer_on_known_groups():
 def pool_struct(**changes):
     p = dict(base=1 << 20, page_stride=2 * 16 * 72, head_stride=16 * 72, pages=4, kv_heads=2, head_dim=64, page_size=16)
     p.update(changes)
-    return _Kv4Pool(**p)
+    return C.byref(kv4._Kv4Pool(**p))
+
+
+def tokens_struct(**changes):
+    t = dict(k=1 << 20, v=1 << 21, slots=1 << 20, tokens=3, k_token_stride=128, k_head_stride=64, v_token_stride=128,
+             v_head_stride=64, dtype=0, reserved=0)
+    t.update(changes)
+    return C.byref(kv4._Kv4Tokens(**t))
 
 
 def refused(status, text, code=INVALID):
@@ -59,9 +66,8 @@ def refused(status, text, code=INVALID):
     (dict(head_stride=16 * 72 - 16), "head_stride", INVALID), (dict(page_stride=16), "page_stride", INVALID)])
 def test_pool_refusals(changes, text, code):
     L, p = mb._L(), pool_struct(**changes)
-    x = 1 << 20
-    refused(L.ms_kv4_append(p, x, x, 0, 3, 128, 64, 128, 64, x, -1, None), text, code)
-    refused(L.ms_kv4_read(p, x, x, 0, 3, 128, 64, 128, 64, x, -1, None), text, code)
+    refused(L.ms_kv4_append(p, tokens_struct(), -1, None), text, code)
+    refused(L.ms_kv4_read(p, tokens_struct(), -1, None), text, code)
     refused(L.ms_kv4_attention(p, attention_struct(), None, 0, -1, None), text, code)
     assert L.ms_kv4_attention_workspace(p, attention_struct()) == -1
 
@@ -71,7 +77,7 @@ def attention_struct(**changes):
              out_head_stride=64, block_table=1 << 20, table_stride=4, lens=1 << 20, cu_q=None, dtype=0, heads=4, rows=3,
              width=4, max_q=1, causal=1, scale=0.0, reserved=0)
     a.update(changes)
-    return _Kv4AttentionArgs(**a)
+    return C.byref(kv4._Kv4AttentionArgs(**a))
 
 
 @pytest.mark.parametrize("changes,text", [
@@ -88,25 +94,35 @@ def test_empty_calls_do_nothing():
     L, p = mb._L(), pool_struct()
     for changes in (dict(rows=0), dict(q_tokens=0, cu_q=1 << 20), dict(max_q=0, cu_q=1 << 20)):
         assert L.ms_kv4_attention(p, attention_struct(**changes), None, 0, -1, None) == 0
-    assert L.ms_kv4_append(p, None, None, 0, 0, 0, 0, 0, 0, None, -1, None) == 0
-    assert L.ms_kv4_read(p, None, None, 2, 0, 0, 0, 0, 0, None, -1, None) == 0
+    none = tokens_struct(k=None, v=None, slots=None, tokens=0)
+    assert L.ms_kv4_append(p, none, -1, None) == 0
+    assert L.ms_kv4_read(p, none, -1, None) == 0
+    assert L.ms_kv4_append(pool_struct(pages=0, base=None), tokens_struct(), -1, None) == 0
 
 
-def test_store_and_table_refusals():
-    L, p, x = mb._L(), pool_struct(), 1 << 20
-    refused(L.ms_kv4_append(p, x, x, 5, 3, 128, 64, 128, 64, x, -1, None), "dtype")
-    refused(L.ms_kv4_append(p, None, x, 0, 3, 128, 64, 128, 64, x, -1, None), "null k")
-    refused(L.ms_kv4_append(p, x, x + 1, 1, 3, 128, 64, 128, 64, x, -1, None), "aligned")
-    refused(L.ms_kv4_append(p, x, x, 0, -3, 128, 64, 128, 64, x, -1, None), "negative")
-    refused(L.ms_kv4_append(None, x, x, 0, 3, 128, 64, 128, 64, x, -1, None), "null pool")
+@pytest.mark.parametrize("changes,text", [
+    (dict(dtype=5), "dtype"), (dict(k=None), "null k"), (dict(v=None), "null k"), (dict(slots=None), "null k"),
+    (dict(v=(1 << 20) + 1, dtype=1), "aligned"), (dict(tokens=-3), "negative")])
+def test_store_refusals(changes, text):
+    L, p = mb._L(), pool_struct()
+    refused(L.ms_kv4_append(p, tokens_struct(**changes), -1, None), text)
+    refused(L.ms_kv4_read(p, tokens_struct(**changes), -1, None), text)
+    refused(L.ms_kv4_append(None, tokens_struct(), -1, None), "null pool")
+    refused(L.ms_kv4_append(p, None, -1, None), "null tokens")
 
-    def tables(lengths=x, new=x, rows=3, page=16, free=x, n_free=9, table=x, width=4, stride=4, slots=x, n_slots=7, cu=x, counts=x):
-        return L.ms_kv_block_tables(lengths, new, rows, page, free, n_free, table, width, stride, slots, n_slots, cu, counts, -1, None)
-    for kw, text in ((dict(lengths=None), "null lengths"), (dict(rows=-1), "negative"), (dict(page=0), "page_size"),
-                     (dict(table=None), "null block_table"), (dict(stride=3), "table_stride"), (dict(slots=None), "null slots"),
-                     (dict(n_slots=1 << 31), "n_slots"), (dict(cu=None), "null cu_new"), (dict(counts=None), "null cu_new"),
-                     (dict(n_free=-1), "negative")):
-        refused(tables(**kw), text)
+
+@pytest.mark.parametrize("changes,text", [
+    (dict(lengths=None), "null lengths"), (dict(new_tokens=None), "null lengths"), (dict(rows=-1), "negative"),
+    (dict(page_size=0), "page_size"), (dict(block_table=None), "null block_table"), (dict(table_stride=3), "table_stride"),
+    (dict(slots=None), "null slots"), (dict(n_slots=1 << 31), "n_slots"), (dict(cu_new=None), "null cu_new"),
+    (dict(counts=None), "null cu_new"), (dict(n_free=-1), "negative")])
+def test_table_refusals(changes, text):
+    x = 1 << 20
+    t = dict(lengths=x, new_tokens=x, free_pages=x, block_table=x, slots=x, cu_new=x, counts=x, table_stride=4, n_slots=7,
+             rows=3, width=4, page_size=16, n_free=9)
+    t.update(changes)
+    refused(mb._L().ms_kv_block_tables(C.byref(kv4._KvTables(**t)), -1, None), text)
+    refused(mb._L().ms_kv_block_tables(None, -1, None), "null arguments")
 
 
 def test_python_refusals():
@@ -132,5 +148,11 @@ def test_python_refusals():
 
 def test_structs_have_the_library_layout():
     L = mb._L()
-    for name, cls in (("ms_kv4_pool", _Kv4Pool), ("ms_kv4_attention_args", _Kv4AttentionArgs)):
-        assert L.ms_struct_size(name.encode()) == C.sizeof(cls)
+    packs = {"ms_kv_tables": kv4._TABLES, "ms_kv4_pool": kv4._POOL, "ms_kv4_tokens": kv4._TOKENS,
+             "ms_kv4_attention_args": kv4._ATTENTION}
+    for name, cls in kv4.STRUCTS:
+        size = C.sizeof(cls)
+        assert L.ms_struct_size(name.encode()) == size
+        # the packed form the calls pass: every field at its place
+        values = [float(i + 1) if t is C.c_float else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+        assert packs[name](*values).ljust(size, b"\0") == bytes(cls(*values))
