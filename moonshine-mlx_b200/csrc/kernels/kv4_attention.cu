@@ -1,4 +1,6 @@
 // How attention over the 4-bit K/V pages is cut into CTAs (kernels: kv4_attention.cuh).
+#include <climits>
+
 #include "kv4_attention.cuh"
 
 namespace msb {
@@ -10,16 +12,22 @@ AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
     const long long rows = (long long)a.max_q * (a.heads / pool.kv_heads);
     const int most = kv4_groups(pool.head_dim) == 1 && a.dtype != KV4_F32 ? 32 : 16;
     sp.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || most == 16 ? 16 : 32;
-    const long long ctas = (rows + sp.rows - 1) / sp.rows * pool.kv_heads * a.rows;
+    const long long per_row = (rows + sp.rows - 1) / sp.rows * pool.kv_heads, pairs = per_row * a.rows;
+    sp.per_row = (int)std::min(per_row, (long long)INT_MAX);
     const long long width = (long long)a.width * pool.page_size;
-    // positions per CTA: the whole work over about four CTAs per SM, in steps of the four
-    // warps' 256 positions, at least 1024 (a shorter chunk costs more in joining than it
-    // saves) and at most 4096 (a long row beside short ones still spreads)
-    long long chunk = (ctas * width + 4 * 148 - 1) / (4 * 148);
-    chunk = std::min(4096ll, std::max(1024ll, (chunk + 255) / 256 * 256));
-    sp.chunk = (int)chunk;
-    sp.splits = (int)std::max(1ll, (width + chunk - 1) / chunk);
-    sp.warps = 4;
+    // eight warps per CTA when there are fewer CTAs than half the GPU holds, two when there are
+    // several waves of them (less to join and to wait for)
+    sp.warps = pairs < 148 && sp.rows <= 8 ? 8 : pairs > 2 * 592 && sp.rows <= 8 ? 2 : 4;
+    // What one CTA would read of a row is cut where the rows are too few to fill the GPU (16
+    // warps per SM): a few pairs into one wave of equal pieces, by the lengths on the device;
+    // more pairs into chunks of 2048, a full GPU's of 4096, for long rows among short ones.  A
+    // CTA costs about 4 us before its first product, so smaller pieces lose.
+    const int slots = 148 * 16 / sp.warps;
+    const bool few = pairs * 8 < slots;
+    sp.ctas = few ? (int)(slots - pairs) : 0;
+    sp.chunk = few ? 512 : pairs < slots ? 2048 : 4096;
+    sp.splits = (int)std::max(1ll, (width + sp.chunk - 1) / sp.chunk);
+    if (few) sp.splits = (int)std::min((long long)sp.splits, sp.ctas / per_row + 1);
     const int tpp = pool.page_size / KV4_TILE;
     if ((tpp & (tpp - 1)) == 0)
         while (1 << (sp.page_shift + 1) <= tpp) ++sp.page_shift;
@@ -36,6 +44,7 @@ size_t kv4_attention_workspace(const Kv4Pool& pool, const Kv4Attention& a) {
 
 cudaError_t launch_kv4_attention(const Kv4Pool& pool, const Kv4Attention& a, void* workspace, cudaStream_t s) {
     AttSplit sp = split_of(pool, a);
+    if (sp.per_row > 65535) return cudaErrorInvalidConfiguration;
     sp.part = reinterpret_cast<float*>(workspace);
     if (a.dtype == KV4_F32) return launch_kv4_attention_f32(pool, a, sp, s);
     if (a.dtype == KV4_F16) return launch_kv4_attention_f16(pool, a, sp, s);

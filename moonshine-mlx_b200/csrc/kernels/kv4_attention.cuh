@@ -7,7 +7,7 @@
 // and the probabilities.
 //
 // Scores are integer products: the codes as bytes (3 operations per word of 8) times q as fixed
-// point of 15 bits (bf16) or 23 bits in 2 or 3 planes of bytes, sums exact (fp32 starts them at
+// point of 16 bits (24 for fp32) in planes of bytes, sums exact (fp32 starts them at
 // -8 sum(q), so that they are those of d and s d q and b sum(q) do not cancel).  For V a nibble becomes fp16 by one AND-OR into the
 // mantissa of 1024 (the odd nibbles in place, as 16 c) and one packed multiply-add, 9 operations
 // per word, after a byte permute, since its fragments want two positions side by side.  (fp16
@@ -23,6 +23,7 @@
 // that share a long context by a second kernel.
 #pragma once
 
+#include <climits>
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -32,8 +33,10 @@ namespace msb {
 struct AttSplit {
     int warps = 4;           // per CTA
     int rows = 4;            // (token, head) rows per CTA
-    int chunk = 0;           // positions per CTA
-    int splits = 1;          // CTAs along the positions (of the longest row)
+    int per_row = 1;         // CTAs of one batch row along its heads and queries
+    int splits = 1;          // CTAs along the positions at most
+    int chunk = 0;           // positions per CTA at least
+    int ctas = 0;            // > 0: CTAs to cut the positions of all rows into
     int page_shift = -1;     // log2 of a page's tiles, -1 if it is no power of two
     float* part = nullptr;   // [splits][tokens * heads][head_dim], then their (max, sum)
 };
@@ -162,6 +165,20 @@ struct Row {
         return a.causal ? max(0, min(len, len - n + i + 1)) : len;
     }
 };
+// Positions per CTA.  With sp.ctas the positions of all rows over so many, so that a few long
+// rows fill the GPU in one wave of about equal CTAs: the lengths are on the device, and every
+// warp sums them up for itself.
+__device__ __forceinline__ int chunk_of(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp) {
+    if (sp.splits == 1) return INT_MAX;
+    if (sp.ctas == 0) return sp.chunk;
+    const int most = (int)min((long long)a.width * pool.page_size, (long long)INT_MAX);
+    unsigned long long sum = 0;
+    for (int b = threadIdx.x & 31; b < a.rows; b += 32) sum += (unsigned)min(max(0, a.lens[b]), most);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
+    const unsigned long long each = (sum * sp.per_row + sp.ctas - 1) / sp.ctas;
+    return (int)max((unsigned long long)sp.chunk, min(each, 1ull << 30));
+}
 __device__ __forceinline__ int splits_of(int end, int chunk) { return end <= chunk ? 1 : (end + chunk - 1) / chunk; }
 __device__ __forceinline__ int over(int n, int d) { return d == 1 ? n : n / d; }  // d == 1 for most models' heads
 
@@ -170,7 +187,7 @@ __device__ __forceinline__ int over(int n, int d) { return d == 1 ? n : n / d; }
 template <class T, int NG, int NT, int NC>
 struct AttShape {
     static constexpr int ROWS = 4 * NC * NT;
-    static constexpr int QP = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;   // byte planes of q
+    static constexpr int QP = sizeof(T) == 4 ? 3 : 2;                          // byte planes of q
     static constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;   // fp16 planes of the probabilities
     static constexpr int SU = NG == 2 || NT == 4 ? 2 : 4;                      // tiles per ring stage
     static constexpr int QROW = 64 * NG + 8;                                   // bytes per q row, padded
@@ -183,7 +200,7 @@ struct AttShape {
 
 // HD: the head size, or 0 to take it from the pool
 template <class T, int NG, int NT, int NC, int HD>
-__global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention_kernel(const Kv4Pool pool, const Kv4Attention a,
+__global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attention_kernel(const Kv4Pool pool, const Kv4Attention a,
                                                                        const AttSplit sp, int ring_bytes) {
     using S = AttShape<T, NG, NT, NC>;
     constexpr int ROWS = S::ROWS, QP = S::QP, PP = S::PP, SU = S::SU;
@@ -198,13 +215,17 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention
     const int b = blockIdx.z, above = gridDim.y == pool.kv_heads ? 0 : blockIdx.y / pool.kv_heads;
     const int kvh = blockIdx.y - above * pool.kv_heads, row0 = above * ROWS;
     pdl_wait();
+    const int chunk = chunk_of(pool, a, sp);
     const Row row(pool, a, b);
     const int rows = min(ROWS, min(row.n, a.max_q) * per - row0);  // this CTA's (token, head) rows
     if (rows <= 0) return;
     const int end = row.end(a, over(row0 + rows - 1, per)), all_see = row.end(a, over(row0, per));
-    const int first = blockIdx.x * sp.chunk;
-    if ((int)blockIdx.x >= splits_of(end, sp.chunk)) return;
-    const int last = min(end, first + sp.chunk);
+    const int n_split = splits_of(end, chunk);
+    if ((int)blockIdx.x >= n_split) return;
+    // its pieces of equal size, in whole runs
+    constexpr int RUN = SU * KV4_TILE;
+    const int piece = n_split == 1 ? end : ((end + n_split - 1) / n_split + RUN - 1) / RUN * RUN;
+    const int first = min(end, (int)blockIdx.x * piece), last = min(end, first + piece);
     // this warp's runs of SU tiles: wid, wid + W, ... of the chunk
     const int tile0 = first / KV4_TILE, tiles = (last - first + KV4_TILE - 1) / KV4_TILE;
     const int runs = (tiles + SU - 1) / SU;
@@ -245,10 +266,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention
     for (int i = 0; i < ATT_STAGES; ++i)
         if (wid + i * W < runs) fetch(wid + i * W, i);
 
-    // q as fixed point of 8 QP - 1 bits below a power of two, exact for bf16 parts down to 2^-6 of
-    // the row's largest (fp16: 2^-11; fp32: 2^-22 of the largest off), in planes of signed
-    // bytes in fragment order (dims 0 2 4 6, 1 3 5 7 of a word); a negative scale goes into q.  A
-    // q that is not finite makes its row NaN by its factor.
+    // q as fixed point relative to its row's largest, 16 or 24 bits, in planes of signed bytes in
+    // fragment order (dims 0 2 4 6, 1 3 5 7 of a word); a negative scale goes into q.  A q that
+    // is not finite makes its row NaN by its factor.
     int8_t* qb = reinterpret_cast<int8_t*>(smem + ring_bytes);
     constexpr int MAGIC = 0x4b400000;  // 1.5 2^23 as bits: sums onto it read as floats, exact below 2^22
     for (int r = wid; r < ROWS; r += W) {
@@ -266,9 +286,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention
         }
         mx = warp_max(mx);
         odd = __any_sync(FULL, odd);
-        const int e = mx > 0.f && !odd ? min(100, max(-100, ilogbf(mx))) : 0;
-        constexpr int top = 8 * QP - 3;
-        const float up = a.scale < 0.f ? -pow2(top - e) : pow2(top - e);
+        // the largest integer whose bytes are all signed ones, less what rounding may add
+        constexpr float top = QP == 2 ? 32600.f : 8355000.f;
+        const float up = mx > 1e-30f && !odd ? (a.scale < 0.f ? -top : top) / mx : 0.f;
         int sum[NG][QP];
 #pragma unroll
         for (int n = 0; n < NG; ++n)
@@ -277,7 +297,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention
 #pragma unroll
         for (int k = 0; k < 2 * NG; ++k) {
             const int d = lane + 32 * k, i = d & 7, at = (d & ~7) + 4 * (i & 1) + (i >> 1);
-            int v = odd ? 0 : __float2int_rn(fminf(fmaxf(x[k] * up, -8e6f), 8e6f));
+            int v = odd ? 0 : __float2int_rn(x[k] * up);
 #pragma unroll
             for (int pl = 0; pl < QP; ++pl) {  // plane 0 is the lowest byte
                 const int8_t byte = (int8_t)v;
@@ -298,7 +318,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention
             if (lane == 0) s_qs[r][n] = all;
         }
         if (lane == 0) {
-            s_f[r] = odd ? NAN : fmaxf(fabsf(a.scale) * LOG2E * pow2(e - top), 1e-37f);
+            s_f[r] = odd ? NAN : up == 0.f ? 1.f : fmaxf(fabsf(a.scale) * LOG2E / fabsf(up), 1e-37f);
             s_end[r] = real ? row.end(a, qi) : end;
         }
     }
@@ -586,7 +606,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention
         }
     if (W > 1) __syncthreads();
     else __syncwarp();
-    const bool whole = splits_of(end, sp.chunk) == 1;
+    const bool whole = n_split == 1;
     for (int r = wid; r < rows; r += W) {
         float mx = -INFINITY, ls = 0.f;
         for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w][r]);
@@ -619,36 +639,65 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, NT == 1 ? 2 : 1) kv4_attention
     }
 }
 
-// Joins the CTAs of contexts longer than one chunk, in their order: one warp per (token, head).
-template <class T>
-__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const Kv4Pool pool, const Kv4Attention a,
+// Joins the CTAs of contexts longer than one chunk, in their order: eight warps of a CTA on
+// eight (token, head) rows, or all on one (WIDE) when there are many parts, each warp taking
+// every eighth; four parts are loaded at a time.
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4Pool pool, const Kv4Attention a,
                                                                  const AttSplit sp) {
+    __shared__ float s_v[8][128], s_l[8];
     pdl_wait();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, hd = pool.head_dim;
-    const int per = a.heads / pool.kv_heads;
+    const int per = over(a.heads, pool.kv_heads);
+    const int chunk = chunk_of(pool, a, sp);
     const Row row(pool, a, blockIdx.y);
-    const int r = blockIdx.x * 4 + wid, qi = r / a.heads, h = r % a.heads;
+    const int r = WIDE ? blockIdx.x : blockIdx.x * 8 + wid, qi = r / a.heads, h = r % a.heads;
     if (qi >= min(row.n, a.max_q)) return;
-    // the CTA that had this row went by its last row's end
+    // the CTAs that had this row went by their last row's end
     const int in_head = qi * per + h % per, of = min(row.n, a.max_q) * per;
     const int last = min(in_head / sp.rows * sp.rows + sp.rows, of) - 1;
-    const int n = splits_of(row.end(a, last / per), sp.chunk);
+    const int n = splits_of(row.end(a, over(last, per)), chunk);
     if (n == 1) return;
     const long long tok = row.q0 + (long long)qi, each = a.q_tokens * a.heads, at = tok * a.heads + h;
-    const float2* ml = reinterpret_cast<const float2*>(sp.part + sp.splits * each * hd);
+    const float2* ml = reinterpret_cast<const float2*>(sp.part + sp.splits * each * hd) + at;
+    const float* part = sp.part + at * hd;
     float mx = -INFINITY;
-    for (int s = lane; s < n; s += 32) mx = fmaxf(mx, ml[s * each + at].x);
+    for (int s = lane; s < n; s += 32) mx = fmaxf(mx, ml[s * each].x);
     mx = warp_max(mx);
     float v[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
-    for (int s = 0; s < n; ++s) {
-        const float2 x = ml[s * each + at];
-        const float fs = x.x == -INFINITY ? 0.f : ex2(x.x - mx);
-        if (x.y == 0.f) continue;
-        ls = fmaf(x.y, fs, ls);
-        const float* src = sp.part + (s * each + at) * hd;
+    constexpr int STEP = WIDE ? 8 : 1;
+    for (int s0 = WIDE ? wid : 0; s0 < n; s0 += 4 * STEP) {
+        float2 x[4];
+        float y[4][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (lane + 32 * k < hd) v[k] = fmaf(src[lane + 32 * k], fs, v[k]);
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * STEP;
+            x[i] = s < n ? ml[s * each] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                y[i][k] = s < n && lane + 32 * k < hd ? part[s * each * hd + lane + 32 * k] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (x[i].y == 0.f) continue;  // saw nothing
+            const float fs = x[i].x == -INFINITY ? 0.f : ex2(x[i].x - mx);
+            ls = fmaf(x[i].y, fs, ls);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = fmaf(y[i][k], fs, v[k]);
+        }
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s_v[wid][lane + 32 * k] = v[k];
+        if (lane == 0) s_l[wid] = ls;
+        __syncthreads();
+        if (wid) return;
+#pragma unroll
+        for (int w = 1; w < 8; ++w) {
+            ls += s_l[w];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += s_v[w][lane + 32 * k];
+        }
     }
     const float inv = ls == 0.f ? 0.f : 1.f / ls;
     T* out = reinterpret_cast<T*>(a.out) + tok * a.out_token_stride + h * a.out_head_stride;
@@ -667,11 +716,8 @@ cudaError_t launch_shape(const Kv4Pool& pool, const Kv4Attention& a, const AttSp
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    const long long rows = (long long)a.max_q * (a.heads / pool.kv_heads);
-    const long long y = (rows + S::ROWS - 1) / S::ROWS * pool.kv_heads;
-    if (y > 65535) return cudaErrorInvalidConfiguration;
     ++launch_counter();
-    return launch_kernel(fn, dim3(sp.splits, (unsigned)y, a.rows), dim3(32 * sp.warps), smem, s, pool, a, sp,
+    return launch_kernel(fn, dim3(sp.splits, sp.per_row, a.rows), dim3(32 * sp.warps), smem, s, pool, a, sp,
                          (int)S::ring(pool.head_dim, sp.warps));
 }
 
@@ -693,8 +739,16 @@ cudaError_t launch_type(const Kv4Pool& pool, const Kv4Attention& a, const AttSpl
                                       : launch_head<T, 2, 0>(pool, a, sp, s);
     if (e != cudaSuccess || sp.splits == 1) return e;
     ++launch_counter();
-    return launch_kernel(kv4_attention_join_kernel<T>, dim3((unsigned)(((long long)a.max_q * a.heads + 3) / 4), a.rows),
-                         dim3(128), 0, s, pool, a, sp);
+    const bool pdl = pdl_launches();
+    pdl_launches() = true;  // the join waits for the parts in the kernel: its launch overlaps them
+    const long long each = (long long)a.max_q * a.heads;
+    const cudaError_t j =
+        sp.splits > 8 ? launch_kernel(kv4_attention_join_kernel<T, true>, dim3((unsigned)each, a.rows), dim3(256), 0, s,
+                                      pool, a, sp)
+                      : launch_kernel(kv4_attention_join_kernel<T, false>, dim3((unsigned)((each + 7) / 8), a.rows),
+                                      dim3(256), 0, s, pool, a, sp);
+    pdl_launches() = pdl;
+    return j;
 }
 
 }  // namespace
