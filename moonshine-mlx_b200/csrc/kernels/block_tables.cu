@@ -11,7 +11,7 @@
 namespace msb {
 namespace {
 
-constexpr int BT_THREADS = 256;
+constexpr int BT_THREADS = 512;
 constexpr int BT_ITEMS = 4;
 constexpr int BT_CHUNK = BT_THREADS * BT_ITEMS;  // rows per scan step
 
@@ -25,11 +25,19 @@ struct BlockTableArgs {
     int* counts;
     long long n_slots, table_stride;
     int rows, page, n_free, width;
+    int wide;   // slots are 16-byte aligned
+    int shift;  // log2 of the page size, -1 if it is no power of two
     int rows_per_cta;
     long long slots_per_cta;
 };
 
-__device__ __forceinline__ unsigned pages_for(unsigned n, unsigned P) { return n / P + (n % P != 0); }
+__device__ __forceinline__ unsigned over_page(const BlockTableArgs& a, unsigned n) {
+    return a.shift >= 0 ? n >> a.shift : n / (unsigned)a.page;
+}
+__device__ __forceinline__ unsigned pages_for(const BlockTableArgs& a, unsigned n) {
+    const unsigned q = over_page(a, n);
+    return q + (q * (unsigned)a.page != n);
+}
 
 // page number `i` handed out by this call, -1 past the free ones
 __device__ __forceinline__ int fresh_page(const BlockTableArgs& a, unsigned i) {
@@ -62,7 +70,7 @@ __global__ void __launch_bounds__(BT_THREADS) block_tables_kernel(const BlockTab
                 len = max(0, a.lengths[c0 + r]);
                 add = max(0, a.added[c0 + r]);
             }
-            const unsigned have = pages_for((unsigned)len, P), need = pages_for((unsigned)len + (unsigned)add, P);
+            const unsigned have = pages_for(a, (unsigned)len), need = pages_for(a, (unsigned)len + (unsigned)add);
             mine[i] = sum;
             sum += (unsigned long long)(need - have) << 32 | (unsigned)add;
             if (r < nr) s_len[r] = len;
@@ -99,29 +107,45 @@ __global__ void __launch_bounds__(BT_THREADS) block_tables_kernel(const BlockTab
         // table rows [row0, row1) of this chunk: new pages, then -1
         for (int b = max(row0, c0) + wid; b < min(row1, c0 + nr); b += BT_THREADS / 32) {
             const int r = b - c0;
-            const unsigned have = pages_for((unsigned)s_len[r], P), start = (unsigned)s_pg[r];
+            const unsigned have = pages_for(a, (unsigned)s_len[r]), start = (unsigned)s_pg[r];
             const unsigned take = (unsigned)s_pg[r + 1] - start;
             int* t = a.table + b * a.table_stride;
             for (long long k = (long long)have + lane; k < a.width; k += 32)
                 t[k] = k - have < take ? fresh_page(a, start + (unsigned)(k - have)) : -1;
             if (lane == 0) a.cu[b + 1] = s_tok[r + 1];
         }
-        // slots [slot0, slot1) of this chunk's tokens
-        const long long t1 = min(slot1, (long long)s_tok[nr]);
-        for (long long t = max(slot0, (long long)s_tok[0]) + tid; t < t1; t += BT_THREADS) {
-            int lo = 0, hi = nr;  // the last row whose first token is <= t has it
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (s_tok[mid] <= t) lo = mid;
-                else hi = mid;
+        // slots [slot0, slot1) of this chunk's tokens, two per thread (one 16-byte store)
+        const long long t0 = max(slot0, (long long)s_tok[0]), t1 = min(slot1, (long long)s_tok[nr]);
+        int lo = 0;  // the last row whose first token is <= t has it
+        for (long long t = (t0 & ~1ll) + 2 * tid; t < t1; t += 2 * BT_THREADS) {
+            long long slot[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const long long ti = t + i;
+                if (ti < t0 || ti >= t1) continue;
+                if (s_tok[lo + 1] <= ti) {
+                    int hi = nr;
+                    ++lo;
+                    while (hi - lo > 1) {
+                        const int mid = (lo + hi) >> 1;
+                        if (s_tok[mid] <= ti) lo = mid;
+                        else hi = mid;
+                    }
+                }
+                const unsigned len = (unsigned)s_len[lo], pos = len + (unsigned)(ti - s_tok[lo]);
+                const unsigned blk = over_page(a, pos), have = pages_for(a, len);
+                int pg = -1;
+                if (blk < (unsigned)a.width)
+                    pg = blk < have ? a.table[(long long)(c0 + lo) * a.table_stride + blk]
+                                    : fresh_page(a, (unsigned)s_pg[lo] + (blk - have));
+                slot[i] = pg < 0 ? -1ll : (long long)pg * P + (pos - blk * P);
             }
-            const unsigned len = (unsigned)s_len[lo], pos = len + (unsigned)(t - s_tok[lo]), blk = pos / P;
-            const unsigned have = pages_for(len, P);
-            int pg = -1;
-            if (blk < (unsigned)a.width)
-                pg = blk < have ? a.table[(long long)(c0 + lo) * a.table_stride + blk]
-                                : fresh_page(a, (unsigned)s_pg[lo] + (blk - have));
-            a.slots[t] = pg < 0 ? -1ll : (long long)pg * P + pos % P;
+            if (a.wide && t >= t0 && t + 1 < t1) {
+                *reinterpret_cast<longlong2*>(a.slots + t) = make_longlong2(slot[0], slot[1]);
+            } else {
+                if (t >= t0) a.slots[t] = slot[0];
+                if (t + 1 >= t0 && t + 1 < t1) a.slots[t + 1] = slot[1];
+            }
         }
         base = total;
         // done when the scan has passed this CTA's slots and rows (the last CTA writes the sums)
@@ -142,12 +166,15 @@ cudaError_t launch_block_tables(const int* lengths, const int* added, int rows, 
                                 int n_free, int* table, int width, long long table_stride, long long* slots,
                                 long long n_slots, int* cu, int* counts, cudaStream_t s) {
     BlockTableArgs a{lengths, added, free_pages, table, slots, cu, counts, n_slots, table_stride,
-                     rows, page, n_free, width, 0, 0};
+                     rows, page, n_free, width, 0, -1, 0, 0};
+    a.wide = !(reinterpret_cast<uintptr_t>(slots) & 15);
+    for (int n = 0; n < 31; ++n)
+        if (1 << n == page) a.shift = n;
     // one CTA per 16 KB of output, at most four per SM of the 148
     const double out = 8.0 * n_slots + 4.0 * rows * (double)width;
     const int grid = (int)std::min(592.0, std::max(1.0, out / 16384.0));
     a.rows_per_cta = (rows + grid - 1) / grid;
-    a.slots_per_cta = (n_slots + grid - 1) / grid;
+    a.slots_per_cta = ((n_slots + grid - 1) / grid + 1) & ~1ll;
     ++launch_counter();
     return launch_kernel(block_tables_kernel, dim3(grid), dim3(BT_THREADS), 0, s, a);
 }
