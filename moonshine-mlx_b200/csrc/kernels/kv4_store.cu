@@ -2,9 +2,9 @@
 //
 // Per group of 64 dims (kv4.cuh): b = fp16(min x), s = fp16(fp32((max x - min x) / 15)), and the
 // code of x is how many of the borders b + (k + 1/2) s, k = 0 .. 14, are <= x, in exact
-// arithmetic: an fp32 quotient decides unless it lies next to a border, where b, s and x in fp64
-// do (b and (k + 1/2) s have 42 bits together).  So the codes do not depend on how the quotient
-// is rounded.
+// arithmetic: an fp32 quotient decides unless it lies next to a border, where the difference of
+// x and the border does, formed without rounding.  So the codes do not depend on how the
+// quotient is rounded.
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -60,27 +60,73 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
     return c;
 }
+// those of 8 elements, two at a time where a register holds two
+__device__ __forceinline__ void range_of(const Raw<float>& r, float& lo, float& hi) {
+    lo = hi = r.get(0);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+        lo = min_nan(lo, r.get(e));
+        hi = max_nan(hi, r.get(e));
+    }
+}
+template <class T>
+__device__ __forceinline__ void range_of(const Raw<T>& r, float& lo, float& hi) {
+    using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    const T2* p = reinterpret_cast<const T2*>(r.v);
+    const T2 l = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
+    const T2 h = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+    lo = min_nan(to_f32<T>(l.x), to_f32<T>(l.y));
+    hi = max_nan(to_f32<T>(h.x), to_f32<T>(h.y));
+}
 
 // fp32((hi - lo) / 15), the difference and the quotient each corrected by what its rounding left
 __device__ __forceinline__ float fifteenth(float hi, float lo) {
     const float d = hi - lo, z = d - hi;
     const float e = (hi - (d - z)) + (-lo - z);  // hi - lo = d + e exactly (Knuth's two-sum)
-    const float q = __fdiv_rn(d, 15.f);
+    const float q = d * (1.f / 15.f);
     return fmaf(fmaf(-q, 15.f, d) + e, 1.f / 15.f, q);
 }
 
-// Adds the code of x under scale s (1 / s = inv) and bias b to `word` in 4 bits from the top.
-// The quotient is off by three roundings of a value below 17, so by 2^-18: only one within 2^-12
-// of a border needs the exact comparison.
-__device__ __forceinline__ void add_code(uint32_t& word, float x, float s, float b, float inv) {
-    const float f = fminf(fmaxf((x - b) * inv, 0.f), 15.f);
-    float n = f + 12582912.f;  // rounds f to a whole number, in the low bits
-    const float off = f - (n - 12582912.f);
-    if (fabsf(off) > 0.499755859375f) {
-        const float below = floorf(f);
-        n = 12582912.f + below + ((double)x >= (double)b + ((double)below + 0.5) * (double)s ? 1.f : 0.f);
+// The code of x next to a border, by its definition: f estimates the quotient, so the border in
+// question is b + (floor(f) + 1/2) s.  x - b is d + e exactly (Knuth's two-sum), the border's
+// distance t from b is exact (16 bits), and so is d - t (d and t are within a factor of two), so
+// the last sum has the sign of x - b - t.
+__device__ __forceinline__ uint32_t exact_code(float x, float f, float s, float b) {
+    const float k = floorf(f), t = (k + 0.5f) * s;
+    const float d = x - b, z = d - x, e = (x - (d - z)) + (-b - z);
+    return (uint32_t)fminf((d - t) + e >= 0.f ? k + 1.f : k, 15.f);
+}
+// Out of line: bf16 values meet a border exactly in one of 1250.
+__device__ __noinline__ uint32_t exact_codes(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
+                                             float s, float b, float inv) {
+    const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        word |= exact_code(x[e], __saturatef((x[e] - b) * inv) * 15.f, s, b) << (4 * e);
+    return word;
+}
+
+// The codes of 8 values.  The quotient, as a part of 15 so that its clamp is the multiply's
+// saturation, is off by five roundings of a value up to 15, so by 2^-17: only when one of the 8
+// lies within 2^-16 of a border does the exact comparison decide.
+template <class T>
+__device__ __forceinline__ uint32_t codes_of(const Raw<T>& r, float s, float b) {
+    float inv;  // to 2^-23
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(15.f * s));
+    float x[8], off = 0.f;
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = r.get(e);
+        const float y = __saturatef((x[e] - b) * inv);
+        const float n = fmaf(y, 15.f, 12582912.f);  // 1.5 2^23 and the nearest whole number
+        off = fmaxf(off, fabsf(fmaf(y, 15.f, 12582912.f - n)));
+        word += __float_as_uint(n) << (4 * e);
     }
-    word = (word >> 4) + (__float_as_uint(n) << 28);
+    word -= 0x4b400000u + 0xb4000000u + 0x40000000u;  // the bits of 1.5 2^23, shifted as they were added
+    if (off > 0.499984741f) word = exact_codes(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s, b, inv);
+    return word;
 }
 
 // Where a slot lies: tile word pointer of the head and position in the tile
@@ -110,10 +156,9 @@ struct Tokens {
     }
 };
 
-// One warp per (16 tokens, head): 8 dims per lane, 8 lanes per group of 64, 4 tokens at a time,
-// all loads first.  Bound by HBM for prompts: about 14 operations per element against 13 that
-// the issue rate allows at copy bandwidth.  A whole tile goes out through shared memory in
-// 16-byte stores; tokens that lie elsewhere (a decode step's) word by word.
+// One warp per (16 tokens, head): 16 dims (two words) per lane, 4 lanes per group of 64, 8 tokens
+// at a time.  A whole tile goes out through shared memory in 16-byte stores; tokens that lie
+// elsewhere (a decode step's) word by word.
 template <class T>
 __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4Pool pool, const T* __restrict__ k,
                                                                       const T* __restrict__ v, long long kst,
@@ -123,7 +168,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
                                                                       int page_shift) {
     __shared__ __align__(16) uint32_t s_tile[STORE_WARPS][STORE_TILE];
     pdl_wait();
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, sub = lane & 7, of4 = lane >> 3;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, sub = lane & 3, of8 = lane >> 2;
     const int hd = pool.head_dim, nw = kv4_words(hd), ng = kv4_groups(hd), H = pool.kv_heads;
     const long long unit = (long long)blockIdx.x * STORE_WARPS + wid, block = unit / H;
     const int h = (int)(unit - block * H);
@@ -131,63 +176,58 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
     if (first >= tokens) return;
     const Tokens t(pool, slots, first, tokens);
     uint32_t* out = s_tile[wid];
-    for (int n = 0; n < ng; ++n) {
-        const int w = 8 * n + sub;
-        Raw<T> raw[2][4];
+#pragma unroll 1
+    for (int part = 0; part < 2 * ng; ++part) {
+        const int kv = part & 1, n = part >> 1, w = 8 * n + 2 * sub, have = min(2, nw - w);  // words of this lane
+        const long long step = kv ? vst : kst;
+        const T* src = (kv ? v + h * vsh : k + h * ksh) + 8 * w + (first + of8) * step;
+        Raw<T> raw[2][2];
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
+        for (int i = 0; i < 2; ++i)
+            if (first + of8 + 8 * i < tokens) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const long long tok = first + 4 * i + of4;
-                const bool mine = tok < tokens && w < nw;
-                if (mine) raw[kv][i].load((kv ? v + tok * vst + h * vsh : k + tok * kst + h * ksh) + 8 * w, wide != 0);
+                for (int j = 0; j < 2; ++j)
+                    if (j < have) raw[i][j].load(src + 8 * i * step + 8 * j, wide != 0);
             }
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = 4 * i + of4;
-                const bool mine = first + at < tokens && w < nw;
-                float lo = INFINITY, hi = -INFINITY;
-                if (mine) {
-                    lo = hi = raw[kv][i].get(0);
-#pragma unroll
-                    for (int e = 1; e < 8; ++e) {
-                        lo = min_nan(lo, raw[kv][i].get(e));
-                        hi = max_nan(hi, raw[kv][i].get(e));
-                    }
-                }
-#pragma unroll
-                for (int o = 4; o > 0; o >>= 1) {
-                    lo = min_nan(lo, __shfl_xor_sync(FULL, lo, o));
-                    hi = max_nan(hi, __shfl_xor_sync(FULL, hi, o));
-                }
-                const bool nan = lo != lo;
-                lo = fminf(fmaxf(lo, -65504.f), 65504.f);
-                hi = fminf(fmaxf(hi, -65504.f), 65504.f);
-                const __half sh = __float2half_rn(fifteenth(hi, lo));
-                const __half bh = nan ? __ushort_as_half(0x7fff) : __float2half_rn(lo);
-                const float s = __half2float(sh), b = __half2float(bh);
-                uint32_t word = 0;
-                if (mine && s > 0.f && !nan) {
-                    const float inv = 1.f / s;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) add_code(word, raw[kv][i].get(e), s, b, inv);
-                }
-                const uint32_t meta = (uint32_t)__half_as_ushort(sh) | (uint32_t)__half_as_ushort(bh) << 16;
-                if (t.whole) {
-                    if (w < nw) out[kv ? kv4_v_word(nw, w, at) : kv4_k_word(nw, w, at)] = word;
-                    if (sub == 0) out[kv4_meta_word(nw, n, at, kv)] = meta;
-                } else {
-                    const long long slot = __shfl_sync(FULL, t.slot, at);
-                    if (slot >= 0) {
-                        int r;
-                        uint32_t* tile = tile_at(pool, page_shift, slot, h, r);
-                        if (w < nw) tile[kv ? kv4_v_word(nw, w, r) : kv4_k_word(nw, w, r)] = word;
-                        if (sub == 0) tile[kv4_meta_word(nw, n, r, kv)] = meta;
-                    }
-                }
+        for (int i = 0; i < 2; ++i) {
+            const int at = of8 + 8 * i;
+            const bool mine = first + at < tokens;
+            float lo = INFINITY, hi = -INFINITY;
+            if (mine && have > 0) range_of(raw[i][0], lo, hi);
+            if (mine && have > 1) {
+                float l, m;
+                range_of(raw[i][1], l, m);
+                lo = min_nan(lo, l);
+                hi = max_nan(hi, m);
             }
+#pragma unroll
+            for (int o = 2; o > 0; o >>= 1) {
+                lo = min_nan(lo, __shfl_xor_sync(FULL, lo, o));
+                hi = max_nan(hi, __shfl_xor_sync(FULL, hi, o));
+            }
+            const bool nan = lo != lo;
+            lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+            hi = fminf(fmaxf(hi, -65504.f), 65504.f);
+            const __half sh = __float2half_rn(fifteenth(hi, lo));
+            const __half bh = nan ? __ushort_as_half(0x7fff) : __float2half_rn(lo);
+            const float s = __half2float(sh), b = __half2float(bh);
+            const bool real = mine && s > 0.f && !nan;
+            uint32_t* to = out;
+            int r = at;
+            bool put = true;
+            if (!t.whole) {
+                const long long slot = __shfl_sync(FULL, t.slot, at);
+                put = slot >= 0;
+                if (put) to = tile_at(pool, page_shift, slot, h, r);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (put && j < have)
+                    to[kv ? kv4_v_word(nw, w + j, r) : kv4_k_word(nw, w + j, r)] = real ? codes_of(raw[i][j], s, b) : 0u;
+            if (put && sub == 0)
+                to[kv4_meta_word(nw, n, r, kv)] = (uint32_t)__half_as_ushort(sh) | (uint32_t)__half_as_ushort(bh) << 16;
+        }
     }
     if (!t.whole) return;
     __syncwarp();
@@ -205,7 +245,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_read_kernel(const Kv4Poo
                                                                     int page_shift) {
     __shared__ __align__(16) uint32_t s_tile[STORE_WARPS][STORE_TILE];
     pdl_wait();
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, sub = lane & 7, of4 = lane >> 3;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, sub = lane & 3, of8 = lane >> 2;
     const int hd = pool.head_dim, nw = kv4_words(hd), ng = kv4_groups(hd), H = pool.kv_heads;
     const long long unit = (long long)blockIdx.x * STORE_WARPS + wid, block = unit / H;
     const int h = (int)(unit - block * H);
@@ -220,35 +260,38 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_read_kernel(const Kv4Poo
         for (int i = lane; i < kv4_tile_words(hd) / 4; i += 32) reinterpret_cast<uint4*>(in)[i] = __ldcs(tile + i);
         __syncwarp();
     }
-    for (int n = 0; n < ng; ++n) {
-        const int w = 8 * n + sub;
+#pragma unroll 1
+    for (int part = 0; part < 2 * ng; ++part) {
+        const int kv = part & 1, n = part >> 1, w = 8 * n + 2 * sub, have = min(2, nw - w);
+        const long long step = kv ? vst : kst;
+        T* dst = (kv ? v + h * vsh : k + h * ksh) + 8 * w + (first + of8) * step;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv)
+        for (int i = 0; i < 2; ++i) {
+            const int at = of8 + 8 * i;
+            const long long slot = __shfl_sync(FULL, t.slot, at);
+            if (first + at >= tokens || have <= 0) continue;
+            const uint32_t* from = in;
+            int r = at;
+            if (!t.whole && slot >= 0) from = tile_at(pool, page_shift, slot, h, r);
+            const bool there = t.whole || slot >= 0;
+            const uint32_t meta = there ? from[kv4_meta_word(nw, n, r, kv)] : 0u;
+            const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&meta));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = 4 * i + of4;
-                const long long tok = first + at, slot = __shfl_sync(FULL, t.slot, at);
-                if (tok >= tokens || w >= nw) continue;
-                uint32_t word = 0, meta = 0;
-                if (t.whole) {
-                    word = in[kv ? kv4_v_word(nw, w, at) : kv4_k_word(nw, w, at)];
-                    meta = in[kv4_meta_word(nw, n, at, kv)];
-                } else if (slot >= 0) {
-                    int r;
-                    const uint32_t* tile = tile_at(pool, page_shift, slot, h, r);
-                    word = tile[kv ? kv4_v_word(nw, w, r) : kv4_k_word(nw, w, r)];
-                    meta = tile[kv4_meta_word(nw, n, r, kv)];
-                }
-                const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&meta));
+            for (int j = 0; j < 2; ++j) {
+                if (j >= have) continue;
+                const uint32_t word = there ? from[kv ? kv4_v_word(nw, w + j, r) : kv4_k_word(nw, w + j, r)] : 0u;
                 Raw<T> raw;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    // 2^23 + c by its bits, less 2^23
-                    const float c = __uint_as_float(((word >> (4 * e)) & 15u) | 0x4b000000u) - 8388608.f;
-                    raw.set(e, fmaf(sb.x, c, sb.y));
+                for (int e = 0; e < 4; ++e) {
+                    // codes e and e + 4 as fp16: in the mantissa of 1024, less 1024
+                    uint32_t c = ((word >> (4 * e)) & 0x000f000fu) | 0x64006400u;
+                    const float2 f = __half22float2(__hsub2(*reinterpret_cast<const __half2*>(&c), __float2half2_rn(1024.f)));
+                    raw.set(e, fmaf(sb.x, f.x, sb.y));
+                    raw.set(e + 4, fmaf(sb.x, f.y, sb.y));
                 }
-                raw.store((kv ? v + tok * vst + h * vsh : k + tok * kst + h * ksh) + 8 * w, wide != 0);
+                raw.store(dst + 8 * i * step + 8 * j, wide != 0);
             }
+        }
     }
 }
 
