@@ -76,7 +76,13 @@ typedef struct {
                                 Both compute the same greedy loop. */
     int32_t quant_stream;    /* quantized checkpoints, clustered kernel: which weights stream as
                                 codes (MS_QSTREAM_*); ignored otherwise */
-    int32_t reserved[6];
+    int32_t cross_kv_bits;   /* cross-attention K/V of ms_generate_batch's lockstep decode: 0 (default)
+                                in the type of kv_dtype, 4 in 4-bit pages (see the 4-bit paged K/V
+                                cache below; a quarter to a third of the fp16 bytes that every step
+                                reads).  As with fp16, the first decoder call reads the fp32 rows and
+                                every later one the stored ones.  At most 8 heads per K/V
+                                head; other calls (ms_generate, streams) keep kv_dtype */
+    int32_t reserved[5];
 } ms_options;
 
 enum { MS_DECODE_AUTO = 0, MS_DECODE_GRID = 1, MS_DECODE_CLUSTER = 2 };

@@ -136,7 +136,7 @@ using namespace msb;
 extern "C" {
 
 int32_t ms_kv4_position_bytes(int32_t head_dim) {
-    if (head_dim < 8 || head_dim > 128 || head_dim % 8) return 0;
+    if (!kv4_head_dim_ok(head_dim)) return 0;
     return head_dim + 8 * ((head_dim + 63) / 64);
 }
 

@@ -386,7 +386,9 @@ cudaError_t launch_gather_cross(const float* const* src32, const void* const* sr
                                 void* dst16, cudaStream_t s);
 
 // ---------------------------------------------------------------- 4-bit paged K/V cache
-enum Kv4Type { KV4_F32 = 0, KV4_F16 = 1, KV4_BF16 = 2 };
+// KV4_STEP: fp32 queries and the bf16 planes of a GEMM input as the result (the batched decoder
+// step's); products as for bf16, or as for fp32 when lo_off asks for the low plane.
+enum Kv4Type { KV4_F32 = 0, KV4_F16 = 1, KV4_BF16 = 2, KV4_STEP = 3 };
 // Pages of 4-bit keys and values (layout: kv4.cuh); strides in bytes, multiples of 16.
 struct Kv4Pool {
     void* base = nullptr;
@@ -409,6 +411,7 @@ struct Kv4Attention {
     const int* cu_q = nullptr;
     int max_q = 1, causal = 0;
     float scale = 1.f;
+    size_t lo_off = 0;  // KV4_STEP: elements from the high plane to the low one, 0: none
 };
 cudaError_t launch_block_tables(const int* lengths, const int* added, int rows, int page, const int* free_pages,
                                 int n_free, int* table, int width, long long table_stride, long long* slots,
@@ -424,6 +427,7 @@ cudaError_t launch_kv4_read(const Kv4Pool& pool, void* k, void* v, int dtype, lo
 // Workspace bytes of launch_kv4_attention (by sizes alone, not by the lengths on the device).
 size_t kv4_attention_workspace(const Kv4Pool& pool, const Kv4Attention& a);
 cudaError_t launch_kv4_attention(const Kv4Pool& pool, const Kv4Attention& a, void* workspace, cudaStream_t s);
+bool kv4_head_dim_ok(int hd);
 
 // Head-clustered batch-1 decode (one 8-CTA cluster per head, packed per-CTA weight streams).
 struct ClusterGeom {

@@ -36,6 +36,8 @@ AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
 
 }  // namespace
 
+bool kv4_head_dim_ok(int hd) { return hd >= 8 && hd <= 128 && hd % 8 == 0; }
+
 size_t kv4_attention_workspace(const Kv4Pool& pool, const Kv4Attention& a) {
     if (a.rows == 0 || a.q_tokens == 0 || a.max_q == 0) return 0;
     const AttSplit sp = split_of(pool, a);
@@ -48,6 +50,7 @@ cudaError_t launch_kv4_attention(const Kv4Pool& pool, const Kv4Attention& a, voi
     sp.part = reinterpret_cast<float*>(workspace);
     if (a.dtype == KV4_F32) return launch_kv4_attention_f32(pool, a, sp, s);
     if (a.dtype == KV4_F16) return launch_kv4_attention_f16(pool, a, sp, s);
+    if (a.dtype == KV4_STEP) return launch_kv4_attention_step(pool, a, sp, s);
     return launch_kv4_attention_bf16(pool, a, sp, s);
 }
 

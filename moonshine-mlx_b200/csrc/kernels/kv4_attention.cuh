@@ -45,6 +45,7 @@ struct AttSplit {
 cudaError_t launch_kv4_attention_f32(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 cudaError_t launch_kv4_attention_f16(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 cudaError_t launch_kv4_attention_bf16(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
+cudaError_t launch_kv4_attention_step(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 
 #ifdef KV4_ATTENTION_KERNELS
 namespace {
@@ -53,7 +54,13 @@ constexpr int ATT_WARPS = 8;   // most per CTA
 constexpr int ATT_STAGES = 2;   // ring slots per warp
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Element types of the batched decoder step: fp32 queries, bf16 planes of a GEMM input out
+struct Step { float v; };       // products as for bf16
+struct StepSplit { float v; };  // products as for fp32, and the low plane
+
 template <class T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<Step>(Step v) { return v.v; }
+template <> __device__ __forceinline__ float to_f32<StepSplit>(StepSplit v) { return v.v; }
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -61,6 +68,17 @@ template <class T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <class T> constexpr bool is_step = std::is_same<T, Step>::value || std::is_same<T, StepSplit>::value;
+template <class T> constexpr bool is_f32 = std::is_same<T, float>::value || std::is_same<T, StepSplit>::value;
+template <class T> constexpr bool is_bf16 = std::is_same<T, __nv_bfloat16>::value || std::is_same<T, Step>::value;
+
+// element `at` of the result
+template <class T>
+__device__ __forceinline__ void put(const Kv4Attention& a, long long at, float v) {
+    if constexpr (is_step<T>) st_bf16_split(reinterpret_cast<__nv_bfloat16*>(a.out) + at, v, a.lo_off);
+    else reinterpret_cast<T*>(a.out)[at] = from_f32<T>(v);
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -187,8 +205,8 @@ __device__ __forceinline__ int over(int n, int d) { return d == 1 ? n : n / d; }
 template <class T, int NG, int NT, int NC>
 struct AttShape {
     static constexpr int ROWS = 4 * NC * NT;
-    static constexpr int QP = sizeof(T) == 4 ? 3 : 2;                          // byte planes of q
-    static constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;   // fp16 planes of the probabilities
+    static constexpr int QP = is_f32<T> ? 3 : 2;                               // byte planes of q
+    static constexpr int PP = is_bf16<T> ? 1 : 2;                              // fp16 planes of the probabilities
     static constexpr int SU = NG == 2 || NT == 4 ? 2 : 4;                      // tiles per ring stage
     static constexpr int QROW = 64 * NG + 8;                                   // bytes per q row, padded
     static size_t ring(int hd, int warps) {  // lanes of a short group read past the last tile; also the join
@@ -204,7 +222,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
                                                                        const AttSplit sp, int ring_bytes) {
     using S = AttShape<T, NG, NT, NC>;
     constexpr int ROWS = S::ROWS, QP = S::QP, PP = S::PP, SU = S::SU;
-    constexpr bool F32 = std::is_same<T, float>::value;
+    constexpr bool F32 = is_f32<T>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t s_bar[ATT_WARPS][ATT_STAGES];
     __shared__ uint32_t s_ok[ATT_WARPS][ATT_STAGES];
@@ -323,6 +341,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         }
     }
     __syncthreads();
+    pdl_trigger();
     uint32_t qf[QP][NT][2 * NG][2];
     float f[NT][NC], qs[NG][NT][NC];
     int from[NG][QP][NT][NC];  // fp32 only: MAGIC - 8 sum(q)
@@ -625,10 +644,10 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         const int qi = over(row0 + r, per), h = kvh * per + (row0 + r - qi * per);
         const long long tok = row.q0 + (long long)qi;
         if (whole) {
-            T* out = reinterpret_cast<T*>(a.out) + tok * a.out_token_stride + h * a.out_head_stride;
+            const long long out = tok * a.out_token_stride + h * a.out_head_stride;
 #pragma unroll
             for (int k = 0; k < 2 * NG; ++k)
-                if (lane + 32 * k < hd) out[lane + 32 * k] = from_f32<T>(ls != ls ? NAN : v[k] * inv);
+                if (lane + 32 * k < hd) put<T>(a, out + lane + 32 * k, ls != ls ? NAN : v[k] * inv);
         } else {
             const long long each = a.q_tokens * a.heads, at = blockIdx.x * each + tok * a.heads + h;
 #pragma unroll
@@ -700,10 +719,10 @@ __global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4Pool p
         }
     }
     const float inv = ls == 0.f ? 0.f : 1.f / ls;
-    T* out = reinterpret_cast<T*>(a.out) + tok * a.out_token_stride + h * a.out_head_stride;
+    const long long out = tok * a.out_token_stride + h * a.out_head_stride;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        if (lane + 32 * k < hd) out[lane + 32 * k] = from_f32<T>(ls != ls ? NAN : v[k] * inv);
+        if (lane + 32 * k < hd) put<T>(a, out + lane + 32 * k, ls != ls ? NAN : v[k] * inv);
 }
 
 template <class T, int NG, int NT, int NC, int HD>
@@ -725,18 +744,24 @@ template <class T, int NG, int HD>
 cudaError_t launch_head(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s) {
     if (sp.rows == 4) return launch_shape<T, NG, 1, 1, HD>(pool, a, sp, s);
     if (sp.rows == 8) return launch_shape<T, NG, 1, 2, HD>(pool, a, sp, s);
-    if (sp.rows == 16) return launch_shape<T, NG, 2, 2, HD>(pool, a, sp, s);
+    if constexpr (is_step<T>) return cudaErrorInvalidValue;  // one token per row
+    else if (sp.rows == 16) return launch_shape<T, NG, 2, 2, HD>(pool, a, sp, s);
     if constexpr (NG == 1 && sizeof(T) == 2) return launch_shape<T, NG, 4, 2, HD>(pool, a, sp, s);
-    return cudaErrorInvalidConfiguration;
+    return cudaErrorInvalidValue;
 }
 
 template <class T>
 cudaError_t launch_type(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s) {
     const int hd = pool.head_dim;
-    const cudaError_t e = hd == 64    ? launch_head<T, 1, 64>(pool, a, sp, s)
-                          : hd == 128 ? launch_head<T, 2, 128>(pool, a, sp, s)
-                          : hd < 64   ? launch_head<T, 1, 0>(pool, a, sp, s)
-                                      : launch_head<T, 2, 0>(pool, a, sp, s);
+    cudaError_t e = cudaErrorInvalidValue;
+    if constexpr (is_step<T>) {  // the decoder's head sizes
+        if (hd <= 64) e = hd == 64 ? launch_head<T, 1, 64>(pool, a, sp, s) : launch_head<T, 1, 0>(pool, a, sp, s);
+    } else {
+        e = hd == 64    ? launch_head<T, 1, 64>(pool, a, sp, s)
+            : hd == 128 ? launch_head<T, 2, 128>(pool, a, sp, s)
+            : hd < 64   ? launch_head<T, 1, 0>(pool, a, sp, s)
+            : launch_head<T, 2, 0>(pool, a, sp, s);
+    }
     if (e != cudaSuccess || sp.splits == 1) return e;
     ++launch_counter();
     const bool pdl = pdl_launches();

@@ -163,27 +163,97 @@ void BatchEngine::ensure_ws(int B, int T, int Mtot, int maxM) {
 
 // Self-attention K/V pages for this call: row b gets ceil(limits[b] / kKvPage) pages (the
 // positions it can reach), numbered consecutively from 0; the pool grows to the largest call
-// seen and every page returns to it when the call ends.  Table entries past a row's pages
-// are -1 (rows that have reached their limit keep stepping in lockstep; their writes there
-// are dropped).
+// seen and every page returns to it when the call ends.  The table is built on the GPU (rows
+// that hold nothing append limits[b] positions).  Table entries past a row's pages are -1
+// (rows that have reached their limit keep stepping in lockstep; their writes there are
+// dropped).
 void BatchEngine::assign_pages(int B, int T, const std::vector<int>& limits) {
     const Config& c = m.cfg;
     const int KVD = c.kv_heads * c.head_dim;
     table_stride = (T + kKvPage - 1) / kKvPage;
-    std::vector<int> tab((size_t)B * table_stride, -1);
-    int64_t next = 0;
+    kvadd_host.resize(B);  // read by the copy below: it lives until the next call
+    int64_t pages = 0;
     for (int b = 0; b < B; ++b) {
-        const int need = (std::max(limits[b], 1) + kKvPage - 1) / kKvPage;
-        for (int q = 0; q < need && q < table_stride; ++q) tab[(size_t)b * table_stride + q] = (int)next++;
+        kvadd_host[b] = std::max(limits[b], 1);
+        pages += (kvadd_host[b] + kKvPage - 1) / kKvPage;
     }
     const size_t page_bytes = (size_t)c.layers * 2 * KVD * kKvPage * 4;  // fp32-sized: the KV dtype may change
-    grow(kvpool, (size_t)std::max<int64_t>(next, 1) * page_bytes);
-    pages_used = next;
+    grow(kvpool, (size_t)std::max<int64_t>(pages, 1) * page_bytes);
+    pages_used = pages;
     pages_capacity = (int64_t)(kvpool.bytes / page_bytes);
-    grow(ptable, tab.size() * 4);
-    MSB_CUDA(cudaMemcpyAsync(ptable.p, tab.data(), tab.size() * 4, cudaMemcpyHostToDevice, m.stream));
-    // the host vector goes away at return: the copy must have read it
-    MSB_CUDA(cudaStreamSynchronize(m.stream));
+    grow(ptable, (size_t)B * table_stride * 4);
+    grow(kvlen, (size_t)B * 4);
+    grow(kvadd, (size_t)B * 4);
+    grow(kvsum, (size_t)(B + 3) * 4);
+    MSB_CUDA(cudaMemsetAsync(kvlen.p, 0, (size_t)B * 4, m.stream));
+    MSB_CUDA(cudaMemcpyAsync(kvadd.p, kvadd_host.data(), (size_t)B * 4, cudaMemcpyHostToDevice, m.stream));
+    MSB_CUDA(launch_block_tables(kvlen.as<int>(), kvadd.as<int>(), B, kKvPage, nullptr, (int)pages, ptable.as<int>(),
+                                 table_stride, table_stride, nullptr, 0, kvsum.as<int>(), kvsum.as<int>() + B + 1,
+                                 m.stream));
+}
+
+Kv4Pool BatchEngine::cross4_pool(int layer) const {
+    const Config& c = m.cfg;
+    Kv4Pool p;
+    p.head_stride = (long long)kCrossPage * ms_kv4_position_bytes(c.head_dim);
+    p.page_stride = p.head_stride * c.kv_heads * c.layers;
+    p.base = reinterpret_cast<char*>(c4pool.p) + (size_t)layer * p.head_stride * c.kv_heads;
+    p.pages = c4pages;
+    p.kv_heads = c.kv_heads;
+    p.head_dim = c.head_dim;
+    p.page_size = kCrossPage;
+    return p;
+}
+
+// One step's cross attention of B rows over the 4-bit pages: fp32 queries, the attention
+// output's bf16 planes.
+Kv4Attention BatchEngine::cross4_args(int B) const {
+    const Config& c = m.cfg;
+    const int HD = c.heads * c.head_dim;
+    Kv4Attention a;
+    a.q = qc.p;
+    a.out = attn.p;
+    a.dtype = KV4_STEP;
+    a.heads = c.heads;
+    a.q_tokens = B;
+    a.q_token_stride = a.out_token_stride = HD;
+    a.q_head_stride = a.out_head_stride = c.head_dim;
+    a.table = c4table.as<int>();
+    a.table_stride = a.width = c4width;
+    a.rows = B;
+    a.lens = frames.as<int>();
+    a.scale = std::pow((float)c.head_dim, -0.5f);
+    a.lo_off = split ? (size_t)Bc * HD : 0;
+    return a;
+}
+
+// The cross K/V of all utterances (cross32) into 4-bit pages of kCrossPage frames, every layer
+// through the one table and slot map; their order is that of the concatenated frames.
+void BatchEngine::store_cross4(int B, int Mtot, int maxM, const std::vector<int>& fr) {
+    const Config& c = m.cfg;
+    const size_t seg = (size_t)c.kv_heads * Mc * c.head_dim;  // one layer's K or V in cross32
+    c4width = (maxM + kCrossPage - 1) / kCrossPage;
+    c4pages = 0;
+    for (int b = 0; b < B; ++b) c4pages += (fr[b] + kCrossPage - 1) / kCrossPage;
+    const size_t page = (size_t)kCrossPage * ms_kv4_position_bytes(c.head_dim) * c.kv_heads * c.layers;
+    grow(c4pool, page * c4pages);
+    grow(c4table, (size_t)B * c4width * 4);
+    grow(c4slots, (size_t)Mtot * 8);
+    grow(kvlen, (size_t)B * 4);
+    grow(kvsum, (size_t)(B + 3) * 4);
+    const Kv4Attention a = cross4_args(B);
+    grow(c4work, std::max<size_t>(kv4_attention_workspace(cross4_pool(0), a), 16));
+    MSB_CUDA(cudaMemcpyAsync(frames.p, fr.data(), (size_t)B * 4, cudaMemcpyHostToDevice, m.stream));
+    MSB_CUDA(cudaMemsetAsync(kvlen.p, 0, (size_t)B * 4, m.stream));
+    MSB_CUDA(launch_block_tables(kvlen.as<int>(), frames.as<int>(), B, kCrossPage, nullptr, c4pages, c4table.as<int>(),
+                                 c4width, c4width, c4slots.as<long long>(), Mtot, kvsum.as<int>(),
+                                 kvsum.as<int>() + B + 1, m.stream));
+    for (int l = 0; l < c.layers; ++l) {
+        const float* k = cross32.as<float>() + (size_t)l * 2 * seg;
+        const long long head = (long long)Mc * c.head_dim;
+        MSB_CUDA(launch_kv4_append(cross4_pool(l), k, k + seg, KV4_F32, Mtot, c.head_dim, head, c.head_dim, head,
+                                   c4slots.as<long long>(), m.stream));
+    }
 }
 
 void BatchEngine::gemm(const CUtensorMap& a, const CUtensorMap& b, TcGemmArgs& ga, int K, int bn,
@@ -303,11 +373,14 @@ void BatchEngine::enqueue_step(int B, int max_frames, bool forced, bool first, f
             fold(ga, L.cs_cq);
             gemm(a_hb, L.m_cq, ga, d, kBnNarrow, hb_lo, wlo(L.m_cq_lo));
         }
-        MSB_CUDA(launch_cross_attn_batch(qc.as<float>(), cross32.as<float>(), m.kv_f16 ? cross16.p : cross32.p,
-                                         m.kv_f16 ? 1 : 0, posp, frame_off.as<int>(), frames.as<int>(), B, H, KVH,
-                                         hd, Mc, l, max_frames, scale, part.as<float>(), attn.as<__nv_bfloat16>(),
-                                         first ? 1 : 0, status.as<unsigned>(), s, lo_attn,
-                                         xrows_on ? &xrows : nullptr));
+        if (cross4 && !first)
+            MSB_CUDA(launch_kv4_attention(cross4_pool(l), cross4_args(B), c4work.p, s));
+        else
+            MSB_CUDA(launch_cross_attn_batch(qc.as<float>(), cross32.as<float>(), m.kv_f16 ? cross16.p : cross32.p,
+                                             m.kv_f16 ? 1 : 0, posp, frame_off.as<int>(), frames.as<int>(), B, H, KVH,
+                                             hd, Mc, l, max_frames, scale, part.as<float>(), attn.as<__nv_bfloat16>(),
+                                             first ? 1 : 0, status.as<unsigned>(), s, lo_attn,
+                                             xrows_on ? &xrows : nullptr));
         {
             TcGemmArgs ga;
             ga.M = B;
@@ -627,7 +700,7 @@ bool BatchEngine::encode_tc(const std::vector<const float*>& audio_dev, const st
     ga.N = c.layers * 2 * c.kv_heads * c.head_dim;
     ga.ep.kv_scatter = 1;
     ga.ep.kv_out32 = cross32.as<float>();
-    ga.ep.kv_out16 = m.kv_f16 ? cross16.p : nullptr;
+    ga.ep.kv_out16 = m.kv_f16 && !cross4 ? cross16.p : nullptr;
     ga.ep.kv_heads = c.kv_heads;
     ga.ep.head_dim = c.head_dim;
     ga.ep.frame_cap = Mc;
@@ -833,10 +906,17 @@ BatchEngine::Result BatchEngine::run(const std::vector<const float*>& audio_dev,
     // the status word starts at zero before any of this call's kernels (the split-K
     // epilogues read it; the decode reports what encoder or decode recorded in it)
     MSB_CUDA(cudaMemsetAsync(status.p, 0, 16, s));
+    struct Cross4Scope {  // for this call only: streams and single utterances read cross16
+        bool& on;
+        Cross4Scope(bool& flag, bool want) : on(flag) { on = want; }
+        ~Cross4Scope() { on = false; }
+    } cross4_scope(cross4, m.opts.cross_kv_bits == 4);
     if (!((m.enc_bf16 || m.opts.weight_dtype == MS_W_AUTO) && encode_tc(audio_dev, n_samples, off, fr))) {
         encode_all(audio_dev, n_samples, off);
-        m.cross_kv_into(memory.as<float>(), Mtot, 0, cross32.as<float>(), m.kv_f16 ? cross16.p : nullptr, Mc);
+        m.cross_kv_into(memory.as<float>(), Mtot, 0, cross32.as<float>(), m.kv_f16 && !cross4 ? cross16.p : nullptr,
+                        Mc);
     }
+    if (cross4) store_cross4(B, Mtot, maxM, fr);
     MSB_CUDA(cudaEventRecord(m.ev[1], s));
     return decode_prepared(B, T, maxM, off, fr, limits, forced, want_logits);
 }

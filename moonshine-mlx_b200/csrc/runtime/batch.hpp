@@ -110,7 +110,19 @@ struct BatchEngine {
     // paged self-attention K/V: page pool and per-row page table of the current call
     DevBuf kvpool, ptable;
     int table_stride = 0;
+    DevBuf kvlen, kvadd, kvsum;       // inputs and sums of the block-table kernel
+    std::vector<int> kvadd_host;
     void assign_pages(int B, int T, const std::vector<int>& limits);
+    // cross K/V in 4-bit pages (ms_options.cross_kv_bits, run() only): one pool
+    // [page][layer][K/V head], a table over the utterances' frames, read from the second
+    // decoder call on
+    static constexpr int kCrossPage = 64;  // frames per page
+    bool cross4 = false;                   // the current call's cross K/V are in 4 bits
+    DevBuf c4pool, c4table, c4slots, c4work;
+    int c4pages = 0, c4width = 0;
+    Kv4Pool cross4_pool(int layer) const;
+    Kv4Attention cross4_args(int B) const;
+    void store_cross4(int B, int Mtot, int maxM, const std::vector<int>& fr);
     CUtensorMap a_hb, a_attn, a_g, a_hb_lo, a_attn_lo, a_g_lo;
 
     // Utterances are encoded concurrently on the model's encoder lanes.

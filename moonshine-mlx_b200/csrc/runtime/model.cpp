@@ -521,6 +521,8 @@ Model* load_model(const std::string& dir, const ms_options& o) {
     m->opts = o;
     m->device = o.device;
     m->kv_f16 = o.kv_dtype == MS_KV_F16;
+    if (o.cross_kv_bits != 0 && o.cross_kv_bits != 4)
+        throw MsError(MS_ERR_INVALID_ARG, "cross_kv_bits must be 0 or 4");
     int ndev = 0;
     MSB_CUDA(cudaGetDeviceCount(&ndev));
     if (o.device < 0 || o.device >= ndev) throw MsError(MS_ERR_INVALID_ARG, "bad device ordinal");
@@ -531,6 +533,8 @@ Model* load_model(const std::string& dir, const ms_options& o) {
     m->num_sms = prop.multiProcessorCount;
     m->cfg = Config::from_json_file(dir + "/config.json");
     validate(m->cfg);
+    if (o.cross_kv_bits == 4 && m->cfg.heads / m->cfg.kv_heads > 8)
+        throw MsError(MS_ERR_UNSUPPORTED, "cross_kv_bits = 4 needs at most 8 heads per K/V head");
     MSB_CUDA(cudaStreamCreateWithFlags(&m->stream, cudaStreamNonBlocking));
     for (auto& e : m->ev) MSB_CUDA(cudaEventCreate(&e));
 

@@ -49,7 +49,7 @@ class MoonshineError(RuntimeError):
 class _Options(C.Structure):
     _fields_ = [("device", C.c_int32), ("kv_dtype", C.c_int32), ("weight_dtype", C.c_int32),
                 ("max_batch", C.c_int32), ("decode_kernel", C.c_int32), ("quant_stream", C.c_int32),
-                ("reserved", C.c_int32 * 6)]
+                ("cross_kv_bits", C.c_int32), ("reserved", C.c_int32 * 5)]
 
 
 class _GenParams(C.Structure):
@@ -364,7 +364,7 @@ class MoonshineModel:
 
     @staticmethod
     def load(path: str, device: int = 0, kv_fp16: bool = True, decode_kernel: str = "auto",
-             weight_dtype: str = "auto", quant_stream: str = "auto") -> "MoonshineModel":
+             weight_dtype: str = "auto", quant_stream: str = "auto", cross_kv_bits: int = 0) -> "MoonshineModel":
         """MoonshineModel.load(from:) for a local directory (MoonshineModel.swift:409-414).
 
         ``decode_kernel`` picks the batch-1 decode kernel: "auto" or "cluster" (one 8-CTA
@@ -373,7 +373,8 @@ class MoonshineModel:
         ms_weight_dtype: "f32" also makes the clustered kernel stream a quantized
         checkpoint's rows dequantized instead of as codes.  ``quant_stream`` ("auto", "all",
         "lm", "none") is MS_QSTREAM_*: which weights of a quantized checkpoint the clustered
-        kernel streams as codes."""
+        kernel streams as codes.  ``cross_kv_bits`` 4 holds the cross-attention K/V of
+        generate_batch in 4-bit pages (0: in the K/V cache's type)."""
         kinds = {"auto": 0, "grid": 1, "cluster": 2}
         if decode_kernel not in kinds:
             raise ValueError("decode_kernel must be one of " + ", ".join(kinds))
@@ -390,6 +391,9 @@ class MoonshineModel:
         if quant_stream not in qkinds:
             raise ValueError("quant_stream must be one of " + ", ".join(qkinds))
         o.quant_stream = qkinds[quant_stream]
+        if cross_kv_bits not in (0, 4):
+            raise ValueError("cross_kv_bits must be 0 or 4")
+        o.cross_kv_bits = cross_kv_bits
         h = C.c_void_p()
         _check(_L().ms_model_load(path.encode(), C.byref(o), C.byref(h)))
         return MoonshineModel(h)
