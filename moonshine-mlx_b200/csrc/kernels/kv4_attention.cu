@@ -8,10 +8,14 @@ namespace {
 
 AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
     AttSplit sp;
-    // rows per CTA: as many as one K/V head has, up to what the registers hold
+    // Rows per CTA: as many as one K/V head has, up to 16, or 128 in the wide kernel, whose stages
+    // take as long for 20 rows as for 128.  Against each other, 32 requests of 4000 positions, 4
+    // K/V heads, bf16: heads of 64, 20 rows 61 (wide) and 59 us, 36 rows 74 and 82, 128 rows 90
+    // and 158; heads of 128, 35 rows 133 and 123, 63 rows 141 and 168, 126 rows 162 and 246.
+    // (fp32 has no wide kernel: its products need more planes.)
     const long long rows = (long long)a.max_q * (a.heads / pool.kv_heads);
-    const int most = kv4_groups(pool.head_dim) == 1 && a.dtype != KV4_F32 ? 32 : 16;
-    sp.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 || most == 16 ? 16 : 32;
+    const bool wide = rows > 16 + 16 * kv4_groups(pool.head_dim) && (a.dtype == KV4_F16 || a.dtype == KV4_BF16);
+    sp.rows = wide ? 128 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
     const long long per_row = (rows + sp.rows - 1) / sp.rows * pool.kv_heads, pairs = per_row * a.rows;
     sp.per_row = (int)std::min(per_row, (long long)INT_MAX);
     const long long width = (long long)a.width * pool.page_size;
@@ -22,7 +26,7 @@ AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
     // warps per SM): a few pairs into one wave of equal pieces, by the lengths on the device;
     // more pairs into chunks of 2048, a full GPU's of 4096, for long rows among short ones.  A
     // CTA costs about 4 us before its first product, so smaller pieces lose.
-    const int slots = 148 * 16 / sp.warps;
+    const int slots = wide ? 148 * 2 : 148 * 16 / sp.warps;
     const bool few = pairs * 8 < slots;
     sp.ctas = few ? (int)(slots - pairs) : 0;
     sp.chunk = few ? 512 : pairs < slots ? 2048 : 4096;
@@ -48,6 +52,7 @@ cudaError_t launch_kv4_attention(const Kv4Pool& pool, const Kv4Attention& a, voi
     AttSplit sp = split_of(pool, a);
     if (sp.per_row > 65535) return cudaErrorInvalidConfiguration;
     sp.part = reinterpret_cast<float*>(workspace);
+    if (sp.rows == 128) return launch_kv4_attention_wide(pool, a, sp, s);
     if (a.dtype == KV4_F32) return launch_kv4_attention_f32(pool, a, sp, s);
     if (a.dtype == KV4_F16) return launch_kv4_attention_f16(pool, a, sp, s);
     if (a.dtype == KV4_STEP) return launch_kv4_attention_step(pool, a, sp, s);

@@ -45,6 +45,7 @@ struct AttSplit {
 cudaError_t launch_kv4_attention_f32(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 cudaError_t launch_kv4_attention_f16(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 cudaError_t launch_kv4_attention_bf16(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
+cudaError_t launch_kv4_attention_wide(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 cudaError_t launch_kv4_attention_step(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 
 #ifdef KV4_ATTENTION_KERNELS
@@ -207,7 +208,7 @@ struct AttShape {
     static constexpr int ROWS = 4 * NC * NT;
     static constexpr int QP = is_f32<T> ? 3 : 2;                               // byte planes of q
     static constexpr int PP = is_bf16<T> ? 1 : 2;                              // fp16 planes of the probabilities
-    static constexpr int SU = NG == 2 || NT == 4 ? 2 : 4;                      // tiles per ring stage
+    static constexpr int SU = NG == 2 ? 2 : 4;                                 // tiles per ring stage
     static constexpr int QROW = 64 * NG + 8;                                   // bytes per q row, padded
     static size_t ring(int hd, int warps) {  // lanes of a short group read past the last tile; also the join
         const size_t r = (size_t)warps * ATT_STAGES * SU * kv4_tile_words(hd) * 4 + 512;
@@ -725,6 +726,21 @@ __global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4Pool p
         if (lane + 32 * k < hd) put<T>(a, out + lane + 32 * k, ls != ls ? NAN : v[k] * inv);
 }
 
+template <class T>
+cudaError_t launch_join(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s) {
+    ++launch_counter();
+    const bool pdl = pdl_launches();
+    pdl_launches() = true;  // the join waits for the parts in the kernel: its launch overlaps them
+    const long long each = (long long)a.max_q * a.heads;
+    const cudaError_t j =
+        sp.splits > 8 ? launch_kernel(kv4_attention_join_kernel<T, true>, dim3((unsigned)each, a.rows), dim3(256), 0, s,
+                                      pool, a, sp)
+                      : launch_kernel(kv4_attention_join_kernel<T, false>, dim3((unsigned)((each + 7) / 8), a.rows),
+                                      dim3(256), 0, s, pool, a, sp);
+    pdl_launches() = pdl;
+    return j;
+}
+
 template <class T, int NG, int NT, int NC, int HD>
 cudaError_t launch_shape(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s) {
     using S = AttShape<T, NG, NT, NC>;
@@ -744,9 +760,8 @@ template <class T, int NG, int HD>
 cudaError_t launch_head(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s) {
     if (sp.rows == 4) return launch_shape<T, NG, 1, 1, HD>(pool, a, sp, s);
     if (sp.rows == 8) return launch_shape<T, NG, 1, 2, HD>(pool, a, sp, s);
-    if constexpr (is_step<T>) return cudaErrorInvalidValue;  // one token per row
-    else if (sp.rows == 16) return launch_shape<T, NG, 2, 2, HD>(pool, a, sp, s);
-    if constexpr (NG == 1 && sizeof(T) == 2) return launch_shape<T, NG, 4, 2, HD>(pool, a, sp, s);
+    if constexpr (!is_step<T>)  // one token per row
+        if (sp.rows == 16) return launch_shape<T, NG, 2, 2, HD>(pool, a, sp, s);
     return cudaErrorInvalidValue;
 }
 
@@ -762,18 +777,7 @@ cudaError_t launch_type(const Kv4Pool& pool, const Kv4Attention& a, const AttSpl
             : hd < 64   ? launch_head<T, 1, 0>(pool, a, sp, s)
             : launch_head<T, 2, 0>(pool, a, sp, s);
     }
-    if (e != cudaSuccess || sp.splits == 1) return e;
-    ++launch_counter();
-    const bool pdl = pdl_launches();
-    pdl_launches() = true;  // the join waits for the parts in the kernel: its launch overlaps them
-    const long long each = (long long)a.max_q * a.heads;
-    const cudaError_t j =
-        sp.splits > 8 ? launch_kernel(kv4_attention_join_kernel<T, true>, dim3((unsigned)each, a.rows), dim3(256), 0, s,
-                                      pool, a, sp)
-                      : launch_kernel(kv4_attention_join_kernel<T, false>, dim3((unsigned)((each + 7) / 8), a.rows),
-                                      dim3(256), 0, s, pool, a, sp);
-    pdl_launches() = pdl;
-    return j;
+    return e != cudaSuccess || sp.splits == 1 ? e : launch_join<T>(pool, a, sp, s);
 }
 
 }  // namespace
