@@ -233,21 +233,6 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     const int hd = HD ? HD : pool.head_dim, nw = kv4_words(hd), P = pool.page_size, per = over(a.heads, pool.kv_heads);
     const int b = blockIdx.z, above = gridDim.y == pool.kv_heads ? 0 : blockIdx.y / pool.kv_heads;
     const int kvh = blockIdx.y - above * pool.kv_heads, row0 = above * ROWS;
-    pdl_wait();
-    const int chunk = chunk_of(pool, a, sp);
-    const Row row(pool, a, b);
-    const int rows = min(ROWS, min(row.n, a.max_q) * per - row0);  // this CTA's (token, head) rows
-    if (rows <= 0) return;
-    const int end = row.end(a, over(row0 + rows - 1, per)), all_see = row.end(a, over(row0, per));
-    const int n_split = splits_of(end, chunk);
-    if ((int)blockIdx.x >= n_split) return;
-    // its pieces of equal size, in whole runs
-    constexpr int RUN = SU * KV4_TILE;
-    const int piece = n_split == 1 ? end : ((end + n_split - 1) / n_split + RUN - 1) / RUN * RUN;
-    const int first = min(end, (int)blockIdx.x * piece), last = min(end, first + piece);
-    // this warp's runs of SU tiles: wid, wid + W, ... of the chunk
-    const int tile0 = first / KV4_TILE, tiles = (last - first + KV4_TILE - 1) / KV4_TILE;
-    const int runs = (tiles + SU - 1) / SU;
     const int tile_words = kv4_tile_words(hd), tpp = P / KV4_TILE;
     const uint32_t tile_bytes = (uint32_t)tile_words * 4;
     unsigned char* ring = smem + (size_t)wid * ATT_STAGES * SU * tile_bytes;
@@ -256,34 +241,68 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     __syncwarp();
     const int* table = a.table + (long long)b * a.table_stride;
     const char* head = reinterpret_cast<const char*>(pool.base) + kvh * pool.head_stride;
-    // Run `run` into ring slot `slot`: lane u stands for tile u of the run; the first tile of
-    // the run and of every page copies the tiles that lie behind one another.
-    auto fetch = [&](int run, int slot) {
+    // Run `run` of the tiles tile0 .. tile0 + tiles - 1: lane u stands for tile u of the run; the
+    // first tile of the run and of every page copies the tiles that lie behind one another.
+    struct Look {
+        int page, in_page, len;  // len 0: nothing to copy
+    };
+    auto look = [&](int tile0, int tiles, int run) {
         const int u0 = run * SU, n = min(SU, tiles - u0);
         const int tile = tile0 + u0 + lane;
         const int nth = sp.page_shift >= 0 ? tile >> sp.page_shift : tile / tpp, in_page = tile - nth * tpp;
         const bool starts = lane < n && (lane == 0 || in_page == 0);
-        int page = -1, len = 0;
-        if (starts) {
-            page = table[nth];
-            if (page < 0 || page >= pool.pages) page = -1;
-            len = min(n - lane, tpp - in_page);
-        }
-        uint32_t ok = page >= 0 ? ((1u << len) - 1) << lane : 0u;
-        ok = __reduce_or_sync(FULL, ok);
+        return Look{starts ? table[nth] : -1, in_page, starts ? min(n - lane, tpp - in_page) : 0};
+    };
+    auto copy = [&](const Look& k, int slot) {
+        const bool there = k.len > 0 && k.page >= 0 && k.page < pool.pages;
+        const uint32_t ok = __reduce_or_sync(FULL, there ? ((1u << k.len) - 1) << lane : 0u);
         if (lane == 0) {
             s_ok[wid][slot] = ok;
             mbar_expect_tx(&s_bar[wid][slot], __popc(ok) * tile_bytes);
         }
         __syncwarp();
-        if (page >= 0)
+        if (there)
             bulk_load(ring + (size_t)(slot * SU + lane) * tile_bytes,
-                      head + page * pool.page_stride + (long long)in_page * tile_bytes, len * tile_bytes,
+                      head + k.page * pool.page_stride + (long long)k.in_page * tile_bytes, k.len * tile_bytes,
                       &s_bar[wid][slot]);
     };
+    pdl_wait();
+    // A CTA that begins at position 0 asks for its first runs by the table alone, whatever the
+    // row's length: one memory latency less (2560 CTAs of one position 18.3 -> 16.4 us; with two
+    // groups the registers it holds cost more than that).  Runs behind the length are waited for.
+    const int whole_row = NG == 1 && sp.splits == 1 && above == 0 ? a.width * tpp : 0;
+    Look ahead[ATT_STAGES];
+    if constexpr (NG == 1)
 #pragma unroll
-    for (int i = 0; i < ATT_STAGES; ++i)
-        if (wid + i * W < runs) fetch(wid + i * W, i);
+        for (int i = 0; i < ATT_STAGES; ++i) ahead[i] = look(0, whole_row, wid + i * W);
+    const int chunk = chunk_of(pool, a, sp);
+    const Row row(pool, a, b);
+    int early = 0;
+    if constexpr (NG == 1)
+#pragma unroll
+        for (int i = 0; i < ATT_STAGES; ++i)
+            if ((wid + i * W) * SU < whole_row) {
+                copy(ahead[i], i);
+                early = i + 1;
+            }
+    const int rows = min(ROWS, min(row.n, a.max_q) * per - row0);  // this CTA's (token, head) rows
+    const int end = rows > 0 ? row.end(a, over(row0 + rows - 1, per)) : 0, all_see = rows > 0 ? row.end(a, over(row0, per)) : 0;
+    const int n_split = splits_of(end, chunk);
+    if (rows <= 0 || (int)blockIdx.x >= n_split) {
+        for (int i = 0; i < early; ++i) mbar_wait(&s_bar[wid][i], 0);
+        return;
+    }
+    // its pieces of equal size, in whole runs
+    constexpr int RUN = SU * KV4_TILE;
+    const int piece = n_split == 1 ? end : ((end + n_split - 1) / n_split + RUN - 1) / RUN * RUN;
+    const int first = min(end, (int)blockIdx.x * piece), last = min(end, first + piece);
+    // this warp's runs of SU tiles: wid, wid + W, ... of the piece
+    const int tile0 = first / KV4_TILE, tiles = (last - first + KV4_TILE - 1) / KV4_TILE;
+    const int runs = (tiles + SU - 1) / SU;
+    if (early == 0)
+#pragma unroll
+        for (int i = 0; i < ATT_STAGES; ++i)
+            if (wid + i * W < runs) copy(look(tile0, tiles, wid + i * W), i);
 
     // q as fixed point relative to its row's largest, 16 or 24 bits, in planes of signed bytes in
     // fragment order (dims 0 2 4 6, 1 3 5 7 of a word); a negative scale goes into q.  A q that
@@ -291,7 +310,22 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     int8_t* qb = reinterpret_cast<int8_t*>(smem + ring_bytes);
     constexpr int MAGIC = 0x4b400000;  // 1.5 2^23 as bits: sums onto it read as floats, exact below 2^22
     for (int r = wid; r < ROWS; r += W) {
-        const bool real = r < rows;
+        if (r >= rows) {
+            for (int k = lane; k < 16 * NG; k += 32)
+#pragma unroll
+                for (int pl = 0; pl < QP; ++pl) *reinterpret_cast<int*>(qb + (pl * ROWS + r) * S::QROW + 4 * k) = 0;
+            if (lane < NG) {
+                s_qs[r][lane] = 0.f;
+#pragma unroll
+                for (int pl = 0; pl < QP; ++pl)
+                    if (F32) s_from[r][lane][pl] = MAGIC;
+            }
+            if (lane == 0) {
+                s_f[r] = 1.f;
+                s_end[r] = end;
+            }
+            continue;
+        }
         const int qi = over(row0 + r, per), h = kvh * per + (row0 + r - qi * per);
         const T* qp = reinterpret_cast<const T*>(a.q) + (row.q0 + (long long)qi) * a.q_token_stride + h * a.q_head_stride;
         float x[2 * NG], mx = 0.f;
@@ -299,7 +333,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 #pragma unroll
         for (int k = 0; k < 2 * NG; ++k) {
             const int d = lane + 32 * k;
-            x[k] = real && d < hd ? to_f32<T>(qp[d]) : 0.f;
+            x[k] = d < hd ? to_f32<T>(qp[d]) : 0.f;
             odd |= !(fabsf(x[k]) < INFINITY);
             mx = fmaxf(mx, fabsf(x[k]));
         }
@@ -338,7 +372,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         }
         if (lane == 0) {
             s_f[r] = odd ? NAN : up == 0.f ? 1.f : fmaxf(fabsf(a.scale) * LOG2E / fabsf(up), 1e-37f);
-            s_end[r] = real ? row.end(a, qi) : end;
+            s_end[r] = row.end(a, qi);
         }
     }
     __syncthreads();
@@ -591,12 +625,15 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         if (ok == (1u << SU) - 1 && (run + 1) * SU <= see) work(std::true_type{}, run, slot, ok);
         else work(std::false_type{}, run, slot, ok);
         __syncwarp();  // every lane has read the slot
-        if (run + ATT_STAGES * W < runs) fetch(run + ATT_STAGES * W, slot);
+        if (run + ATT_STAGES * W < runs) copy(look(tile0, tiles, run + ATT_STAGES * W), slot);
         if (++slot == ATT_STAGES) {
             slot = 0;
             phase ^= 1;
         }
     }
+
+    for (int i = 0; i < early; ++i)
+        if (wid + i * W >= runs) mbar_wait(&s_bar[wid][i], 0);
 
     // join the warps: unnormalised sums in shared memory (the rings are done with)
     if (W > 1) __syncthreads();
