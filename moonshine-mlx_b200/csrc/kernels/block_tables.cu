@@ -170,9 +170,9 @@ cudaError_t launch_block_tables(const int* lengths, const int* added, int rows, 
     a.wide = !(reinterpret_cast<uintptr_t>(slots) & 15);
     for (int n = 0; n < 31; ++n)
         if (1 << n == page) a.shift = n;
-    // one CTA per 16 KB of output, at most four per SM of the 148
+    // one CTA per 16 KB of output, at most three per SM of the 148
     const double out = 8.0 * n_slots + 4.0 * rows * (double)width;
-    const int grid = (int)std::min(592.0, std::max(1.0, out / 16384.0));
+    const int grid = (int)std::min(444.0, std::max(1.0, out / 16384.0));
     a.rows_per_cta = (rows + grid - 1) / grid;
     a.slots_per_cta = ((n_slots + grid - 1) / grid + 1) & ~1ll;
     ++launch_counter();

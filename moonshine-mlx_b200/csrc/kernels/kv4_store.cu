@@ -16,17 +16,14 @@ template <class T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // 8 elements as they lie in memory
 template <class T>
 struct Raw {
     uint4 v[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* p, bool wide) {
-        if (wide) {
+    template <bool WIDE>
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (WIDE) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
         } else {
@@ -35,8 +32,9 @@ struct Raw {
             for (int i = 0; i < 8; ++i) e[i] = p[i];
         }
     }
-    __device__ __forceinline__ void store(T* p, bool wide) const {
-        if (wide) {
+    template <bool WIDE>
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (WIDE) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, v[i]);
         } else {
@@ -46,7 +44,15 @@ struct Raw {
         }
     }
     __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T*>(v)[i]); }
-    __device__ __forceinline__ void set(int i, float x) { reinterpret_cast<T*>(v)[i] = from_f32<T>(x); }
+    __device__ __forceinline__ void set2(int i, float x, float y) {  // elements i (even) and i + 1
+        if constexpr (std::is_same<T, float>::value) {
+            reinterpret_cast<float2*>(v)[i / 2] = make_float2(x, y);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            reinterpret_cast<__half2*>(v)[i / 2] = __floats2half2_rn(x, y);
+        } else {
+            reinterpret_cast<__nv_bfloat162*>(v)[i / 2] = __floats2bfloat162_rn(x, y);
+        }
+    }
 };
 
 // minimum and maximum that are NaN if either is
@@ -96,14 +102,17 @@ __device__ __forceinline__ uint32_t exact_code(float x, float f, float s, float 
     const float d = x - b, z = d - x, e = (x - (d - z)) + (-b - z);
     return (uint32_t)fminf((d - t) + e >= 0.f ? k + 1.f : k, 15.f);
 }
-// Out of line: bf16 values meet a border exactly in one of 1250.
-__device__ __noinline__ uint32_t exact_codes(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
-                                             float s, float b, float inv) {
+// The codes of 8 values, of which some lie next to a border.  Out of line: bf16 values meet
+// borders exactly, one word in 170.
+__device__ __noinline__ uint32_t exact_codes(uint32_t word, float x0, float x1, float x2, float x3, float x4, float x5,
+                                             float x6, float x7, float s, float b, float inv) {
     const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
-    uint32_t word = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        word |= exact_code(x[e], __saturatef((x[e] - b) * inv) * 15.f, s, b) << (4 * e);
+    for (int e = 0; e < 8; ++e) {
+        const float f = __saturatef((x[e] - b) * inv) * 15.f, n = f + 12582912.f;
+        if (fabsf(f - (n - 12582912.f)) > 0.49997f)
+            word = (word & ~(15u << (4 * e))) | exact_code(x[e], f, s, b) << (4 * e);
+    }
     return word;
 }
 
@@ -111,9 +120,7 @@ __device__ __noinline__ uint32_t exact_codes(float x0, float x1, float x2, float
 // saturation, is off by five roundings of a value up to 15, so by 2^-17: only when one of the 8
 // lies within 2^-16 of a border does the exact comparison decide.
 template <class T>
-__device__ __forceinline__ uint32_t codes_of(const Raw<T>& r, float s, float b) {
-    float inv;  // to 2^-23
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(15.f * s));
+__device__ __forceinline__ uint32_t codes_of(const Raw<T>& r, float s, float b, float inv) {
     float x[8], off = 0.f;
     uint32_t word = 0;
 #pragma unroll
@@ -125,7 +132,7 @@ __device__ __forceinline__ uint32_t codes_of(const Raw<T>& r, float s, float b) 
         word += __float_as_uint(n) << (4 * e);
     }
     word -= 0x4b400000u + 0xb4000000u + 0x40000000u;  // the bits of 1.5 2^23, shifted as they were added
-    if (off > 0.499984741f) word = exact_codes(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s, b, inv);
+    if (off > 0.499984741f) word = exact_codes(word, x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s, b, inv);
     return word;
 }
 
@@ -159,12 +166,12 @@ struct Tokens {
 // One warp per (16 tokens, head): 16 dims (two words) per lane, 4 lanes per group of 64, 8 tokens
 // at a time.  A whole tile goes out through shared memory in 16-byte stores; tokens that lie
 // elsewhere (a decode step's) word by word.
-template <class T>
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4Pool pool, const T* __restrict__ k,
                                                                       const T* __restrict__ v, long long kst,
                                                                       long long ksh, long long vst, long long vsh,
                                                                       long long tokens,
-                                                                      const long long* __restrict__ slots, int wide,
+                                                                      const long long* __restrict__ slots,
                                                                       int page_shift) {
     __shared__ __align__(16) uint32_t s_tile[STORE_WARPS][STORE_TILE];
     pdl_wait();
@@ -176,23 +183,22 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
     if (first >= tokens) return;
     const Tokens t(pool, slots, first, tokens);
     uint32_t* out = s_tile[wid];
-#pragma unroll 1
-    for (int part = 0; part < 2 * ng; ++part) {
+    // (whole tile, part): K or V of one group
+    auto work = [&](auto whole, int part) {
+        constexpr bool WHOLE = decltype(whole)::value;
         const int kv = part & 1, n = part >> 1, w = 8 * n + 2 * sub, have = min(2, nw - w);  // words of this lane
         const long long step = kv ? vst : kst;
         const T* src = (kv ? v + h * vsh : k + h * ksh) + 8 * w + (first + of8) * step;
+        const int left = (int)min(tokens - first, (long long)KV4_TILE) - of8;  // tokens from this lane's on
         Raw<T> raw[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (first + of8 + 8 * i < tokens) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (j < have) raw[i][j].load(src + 8 * i * step + 8 * j, wide != 0);
-            }
+            for (int j = 0; j < 2; ++j)
+                if ((WHOLE || left > 8 * i) && j < have) raw[i][j].template load<WIDE>(src + 8 * i * step + 8 * j);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int at = of8 + 8 * i;
-            const bool mine = first + at < tokens;
+            const bool mine = WHOLE || left > 8 * i;
             float lo = INFINITY, hi = -INFINITY;
             if (mine && have > 0) range_of(raw[i][0], lo, hi);
             if (mine && have > 1) {
@@ -212,24 +218,35 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
             const __half sh = __float2half_rn(fifteenth(hi, lo));
             const __half bh = nan ? __ushort_as_half(0x7fff) : __float2half_rn(lo);
             const float s = __half2float(sh), b = __half2float(bh);
-            const bool real = mine && s > 0.f && !nan;
-            uint32_t* to = out;
-            int r = at;
-            bool put = true;
-            if (!t.whole) {
-                const long long slot = __shfl_sync(FULL, t.slot, at);
-                put = slot >= 0;
-                if (put) to = tile_at(pool, page_shift, slot, h, r);
-            }
+            float inv;  // of 15 s, to 2^-23
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(15.f * s));
+            uint32_t word[2] = {0, 0};
+            if (mine && s > 0.f && !nan) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (put && j < have)
-                    to[kv ? kv4_v_word(nw, w + j, r) : kv4_k_word(nw, w + j, r)] = real ? codes_of(raw[i][j], s, b) : 0u;
-            if (put && sub == 0)
-                to[kv4_meta_word(nw, n, r, kv)] = (uint32_t)__half_as_ushort(sh) | (uint32_t)__half_as_ushort(bh) << 16;
+                for (int j = 0; j < 2; ++j)
+                    if (j < have) word[j] = codes_of(raw[i][j], s, b, inv);
+            }
+            const uint32_t meta = (uint32_t)__half_as_ushort(sh) | (uint32_t)__half_as_ushort(bh) << 16;
+            uint32_t* to = out;
+            int r = of8 + 8 * i;
+            if constexpr (!WHOLE) {
+                const long long slot = __shfl_sync(FULL, t.slot, r);
+                if (slot < 0) continue;
+                to = tile_at(pool, page_shift, slot, h, r);
+            }
+            uint32_t* at = to + (kv ? kv4_v_word(nw, w, r) : kv4_k_word(nw, w, r));
+            if (have > 0) at[0] = word[0];
+            if (have > 1) at[kv ? 16 : 2] = word[1];  // the next word of the vector
+            if (sub == 0) to[kv4_meta_word(nw, n, r, kv)] = meta;
         }
+    };
+    if (!t.whole) {
+#pragma unroll 1
+        for (int part = 0; part < 2 * ng; ++part) work(std::false_type{}, part);
+        return;
     }
-    if (!t.whole) return;
+#pragma unroll 1
+    for (int part = 0; part < 2 * ng; ++part) work(std::true_type{}, part);
     __syncwarp();
     int r;
     uint4* tile = reinterpret_cast<uint4*>(tile_at(pool, page_shift, __shfl_sync(FULL, t.slot, 0), h, r));
@@ -237,11 +254,11 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
 }
 
 // The reverse: a whole tile comes in by 16-byte loads.
-template <class T>
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_read_kernel(const Kv4Pool pool, T* __restrict__ k,
                                                                     T* __restrict__ v, long long kst, long long ksh,
                                                                     long long vst, long long vsh, long long tokens,
-                                                                    const long long* __restrict__ slots, int wide,
+                                                                    const long long* __restrict__ slots,
                                                                     int page_shift) {
     __shared__ __align__(16) uint32_t s_tile[STORE_WARPS][STORE_TILE];
     pdl_wait();
@@ -253,46 +270,60 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_read_kernel(const Kv4Poo
     if (first >= tokens) return;
     const Tokens t(pool, slots, first, tokens);
     uint32_t* in = s_tile[wid];
-    if (t.whole) {
-        int r;
-        const uint4* tile =
-            reinterpret_cast<const uint4*>(tile_at(pool, page_shift, __shfl_sync(FULL, t.slot, 0), h, r));
-        for (int i = lane; i < kv4_tile_words(hd) / 4; i += 32) reinterpret_cast<uint4*>(in)[i] = __ldcs(tile + i);
-        __syncwarp();
-    }
-#pragma unroll 1
-    for (int part = 0; part < 2 * ng; ++part) {
+    auto work = [&](auto whole, int part) {
+        constexpr bool WHOLE = decltype(whole)::value;
         const int kv = part & 1, n = part >> 1, w = 8 * n + 2 * sub, have = min(2, nw - w);
         const long long step = kv ? vst : kst;
         T* dst = (kv ? v + h * vsh : k + h * ksh) + 8 * w + (first + of8) * step;
+        const int left = (int)min(tokens - first, (long long)KV4_TILE) - of8;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int at = of8 + 8 * i;
-            const long long slot = __shfl_sync(FULL, t.slot, at);
-            if (first + at >= tokens || have <= 0) continue;
             const uint32_t* from = in;
-            int r = at;
-            if (!t.whole && slot >= 0) from = tile_at(pool, page_shift, slot, h, r);
-            const bool there = t.whole || slot >= 0;
+            int r = of8 + 8 * i;
+            bool there = true;
+            if constexpr (!WHOLE) {
+                const long long slot = __shfl_sync(FULL, t.slot, r);
+                if (left <= 8 * i) continue;
+                there = slot >= 0;
+                if (there) from = tile_at(pool, page_shift, slot, h, r);
+            }
             const uint32_t meta = there ? from[kv4_meta_word(nw, n, r, kv)] : 0u;
             const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&meta));
+            const uint32_t* at = from + (kv ? kv4_v_word(nw, w, r) : kv4_k_word(nw, w, r));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if (j >= have) continue;
-                const uint32_t word = there ? from[kv ? kv4_v_word(nw, w + j, r) : kv4_k_word(nw, w + j, r)] : 0u;
+                const uint32_t word = there ? at[j == 0 ? 0 : kv ? 16 : 2] : 0u;
                 Raw<T> raw;
+                float x[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     // codes e and e + 4 as fp16: in the mantissa of 1024, less 1024
-                    uint32_t c = ((word >> (4 * e)) & 0x000f000fu) | 0x64006400u;
+                    uint32_t c;
+                    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(c) : "r"(word >> (4 * e)), "r"(0x000f000fu), "r"(0x64006400u));
                     const float2 f = __half22float2(__hsub2(*reinterpret_cast<const __half2*>(&c), __float2half2_rn(1024.f)));
-                    raw.set(e, fmaf(sb.x, f.x, sb.y));
-                    raw.set(e + 4, fmaf(sb.x, f.y, sb.y));
+                    x[e] = fmaf(sb.x, f.x, sb.y);
+                    x[e + 4] = fmaf(sb.x, f.y, sb.y);
                 }
-                raw.store(dst + 8 * i * step + 8 * j, wide != 0);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) raw.set2(e, x[e], x[e + 1]);
+                raw.template store<WIDE>(dst + 8 * i * step + 8 * j);
             }
         }
+    };
+    if (!t.whole) {
+#pragma unroll 1
+        for (int part = 0; part < 2 * ng; ++part) work(std::false_type{}, part);
+        return;
     }
+    int r;
+    const uint32_t* tile = tile_at(pool, page_shift, __shfl_sync(FULL, t.slot, 0), h, r);
+    for (int i = 4 * lane; i < kv4_tile_words(hd); i += 128)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(in + i)), "l"(tile + i) : "memory");
+    asm volatile("cp.async.commit_group;\ncp.async.wait_all;\n" ::: "memory");
+    __syncwarp();
+#pragma unroll 1
+    for (int part = 0; part < 2 * ng; ++part) work(std::true_type{}, part);
 }
 
 bool wide_ok(const void* p, long long st, long long sh, int esize) {
@@ -312,38 +343,40 @@ int shift_of(int page) {
 template <class Kernel, class P>
 cudaError_t launch_store(Kernel kernel, const Kv4Pool& pool, P* k, P* v, long long tokens, long long kst, long long ksh,
                          long long vst, long long vsh, const long long* slots, cudaStream_t s) {
-    const int es = (int)sizeof(P);
-    const int wide = wide_ok(k, kst, ksh, es) && wide_ok(v, vst, vsh, es);
     const long long units = (tokens + KV4_TILE - 1) / KV4_TILE * pool.kv_heads;
     const long long grid = (units + STORE_WARPS - 1) / STORE_WARPS;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     ++launch_counter();
     return launch_kernel(kernel, dim3((unsigned)grid), dim3(32 * STORE_WARPS), 0, s, pool, k, v, kst, ksh, vst, vsh,
-                         tokens, slots, wide, shift_of(pool.page_size));
+                         tokens, slots, shift_of(pool.page_size));
 }
 }  // namespace
 
 cudaError_t launch_kv4_append(const Kv4Pool& pool, const void* k, const void* v, int dtype, long long tokens,
                               long long kst, long long ksh, long long vst, long long vsh, const long long* slots,
                               cudaStream_t s) {
-    auto go = [&](auto kernel, auto* type) {
+    auto go = [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        return launch_store(kernel, pool, (const T*)k, (const T*)v, tokens, kst, ksh, vst, vsh, slots, s);
+        const bool wide = wide_ok(k, kst, ksh, sizeof(T)) && wide_ok(v, vst, vsh, sizeof(T));
+        return launch_store(wide ? kv4_append_kernel<T, true> : kv4_append_kernel<T, false>, pool, (const T*)k,
+                            (const T*)v, tokens, kst, ksh, vst, vsh, slots, s);
     };
-    if (dtype == KV4_F32) return go(kv4_append_kernel<float>, (float*)nullptr);
-    if (dtype == KV4_F16) return go(kv4_append_kernel<__half>, (__half*)nullptr);
-    return go(kv4_append_kernel<__nv_bfloat16>, (__nv_bfloat16*)nullptr);
+    if (dtype == KV4_F32) return go((float*)nullptr);
+    if (dtype == KV4_F16) return go((__half*)nullptr);
+    return go((__nv_bfloat16*)nullptr);
 }
 
 cudaError_t launch_kv4_read(const Kv4Pool& pool, void* k, void* v, int dtype, long long tokens, long long kst,
                             long long ksh, long long vst, long long vsh, const long long* slots, cudaStream_t s) {
-    auto go = [&](auto kernel, auto* type) {
+    auto go = [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        return launch_store(kernel, pool, (T*)k, (T*)v, tokens, kst, ksh, vst, vsh, slots, s);
+        const bool wide = wide_ok(k, kst, ksh, sizeof(T)) && wide_ok(v, vst, vsh, sizeof(T));
+        return launch_store(wide ? kv4_read_kernel<T, true> : kv4_read_kernel<T, false>, pool, (T*)k, (T*)v, tokens,
+                            kst, ksh, vst, vsh, slots, s);
     };
-    if (dtype == KV4_F32) return go(kv4_read_kernel<float>, (float*)nullptr);
-    if (dtype == KV4_F16) return go(kv4_read_kernel<__half>, (__half*)nullptr);
-    return go(kv4_read_kernel<__nv_bfloat16>, (__nv_bfloat16*)nullptr);
+    if (dtype == KV4_F32) return go((float*)nullptr);
+    if (dtype == KV4_F16) return go((__half*)nullptr);
+    return go((__nv_bfloat16*)nullptr);
 }
 
 }  // namespace msb
