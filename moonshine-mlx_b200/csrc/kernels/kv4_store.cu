@@ -17,15 +17,19 @@ template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; 
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// 8 elements as they lie in memory
+// 8 elements as they lie in memory: one 16-byte or, for fp32, 32-byte access
 template <class T>
 struct Raw {
     uint4 v[sizeof(T) / 2];
     template <bool WIDE>
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (WIDE) {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        if constexpr (WIDE && sizeof(T) == 4) {
+            asm volatile("ld.global.cs.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z),
+                           "=r"(v[1].w)
+                         : "l"(p));
+        } else if constexpr (WIDE) {
+            v[0] = __ldcs(reinterpret_cast<const uint4*>(p));
         } else {
             T* e = reinterpret_cast<T*>(v);
 #pragma unroll
@@ -34,9 +38,12 @@ struct Raw {
     }
     template <bool WIDE>
     __device__ __forceinline__ void store(T* p) const {
-        if constexpr (WIDE) {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, v[i]);
+        if constexpr (WIDE && sizeof(T) == 4) {
+            asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0].x), "r"(v[0].y),
+                         "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w)
+                         : "memory");
+        } else if constexpr (WIDE) {
+            __stcs(reinterpret_cast<uint4*>(p), v[0]);
         } else {
             const T* e = reinterpret_cast<const T*>(v);
 #pragma unroll
@@ -163,8 +170,8 @@ struct Tokens {
     }
 };
 
-// One warp per (16 tokens, head): 16 dims (two words) per lane, 4 lanes per group of 64, 8 tokens
-// at a time.  A whole tile goes out through shared memory in 16-byte stores; tokens that lie
+// One warp per (16 tokens, head): two words (16 dims) per lane, 4 lanes per group of 64, 8 tokens
+// at a time; the lanes of a vector take neighbouring words, so that a store fills whole sectors.  A whole tile goes out through shared memory in 16-byte stores; tokens that lie
 // elsewhere (a decode step's) word by word.
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4Pool pool, const T* __restrict__ k,
@@ -186,16 +193,19 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
     // (whole tile, part): K or V of one group
     auto work = [&](auto whole, int part) {
         constexpr bool WHOLE = decltype(whole)::value;
-        const int kv = part & 1, n = part >> 1, w = 8 * n + 2 * sub, have = min(2, nw - w);  // words of this lane
+        const int kv = part & 1, n = part >> 1, w = 8 * n + sub, have = nw > w ? nw > w + 4 ? 2 : 1 : 0;  // words w and w + 4
         const long long step = kv ? vst : kst;
         const T* src = (kv ? v + h * vsh : k + h * ksh) + 8 * w + (first + of8) * step;
         const int left = (int)min(tokens - first, (long long)KV4_TILE) - of8;  // tokens from this lane's on
+        // tile words of position of8; 8 positions on they are 1 (K, scales) or 2 (V) further
+        const int at0 = kv ? kv4_v_word(nw, w, of8) : kv4_k_word(nw, w, of8);
+        const int at1 = kv ? at0 + 64 : kv4_k_word(nw, w + 4, of8), at_meta = kv4_meta_word(nw, n, of8, kv);
         Raw<T> raw[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                if ((WHOLE || left > 8 * i) && j < have) raw[i][j].template load<WIDE>(src + 8 * i * step + 8 * j);
+                if ((WHOLE || left > 8 * i) && j < have) raw[i][j].template load<WIDE>(src + 8 * i * step + 32 * j);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const bool mine = WHOLE || left > 8 * i;
@@ -227,17 +237,20 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
                     if (j < have) word[j] = codes_of(raw[i][j], s, b, inv);
             }
             const uint32_t meta = (uint32_t)__half_as_ushort(sh) | (uint32_t)__half_as_ushort(bh) << 16;
-            uint32_t* to = out;
-            int r = of8 + 8 * i;
-            if constexpr (!WHOLE) {
-                const long long slot = __shfl_sync(FULL, t.slot, r);
+            if constexpr (WHOLE) {
+                if (have > 0) out[at0 + (1 + kv) * i] = word[0];
+                if (have > 1) out[at1 + (1 + kv) * i] = word[1];
+                if (sub == 0) out[at_meta + i] = meta;
+            } else {
+                const long long slot = __shfl_sync(FULL, t.slot, of8 + 8 * i);
                 if (slot < 0) continue;
-                to = tile_at(pool, page_shift, slot, h, r);
+                int r;
+                uint32_t* to = tile_at(pool, page_shift, slot, h, r);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (j < have) to[kv ? kv4_v_word(nw, w + 4 * j, r) : kv4_k_word(nw, w + 4 * j, r)] = word[j];
+                if (sub == 0) to[kv4_meta_word(nw, n, r, kv)] = meta;
             }
-            uint32_t* at = to + (kv ? kv4_v_word(nw, w, r) : kv4_k_word(nw, w, r));
-            if (have > 0) at[0] = word[0];
-            if (have > 1) at[kv ? 16 : 2] = word[1];  // the next word of the vector
-            if (sub == 0) to[kv4_meta_word(nw, n, r, kv)] = meta;
         }
     };
     if (!t.whole) {
@@ -272,28 +285,37 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_read_kernel(const Kv4Poo
     uint32_t* in = s_tile[wid];
     auto work = [&](auto whole, int part) {
         constexpr bool WHOLE = decltype(whole)::value;
-        const int kv = part & 1, n = part >> 1, w = 8 * n + 2 * sub, have = min(2, nw - w);
+        const int kv = part & 1, n = part >> 1, w = 8 * n + sub, have = nw > w ? nw > w + 4 ? 2 : 1 : 0;
         const long long step = kv ? vst : kst;
         T* dst = (kv ? v + h * vsh : k + h * ksh) + 8 * w + (first + of8) * step;
         const int left = (int)min(tokens - first, (long long)KV4_TILE) - of8;
+        // tile words of position of8; 8 positions on they are 1 (K, scales) or 2 (V) further
+        const int at0 = kv ? kv4_v_word(nw, w, of8) : kv4_k_word(nw, w, of8);
+        const int at1 = kv ? at0 + 64 : kv4_k_word(nw, w + 4, of8), at_meta = kv4_meta_word(nw, n, of8, kv);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t* from = in;
-            int r = of8 + 8 * i;
-            bool there = true;
-            if constexpr (!WHOLE) {
-                const long long slot = __shfl_sync(FULL, t.slot, r);
+            uint32_t meta = 0, words[2] = {0, 0};
+            if constexpr (WHOLE) {
+                meta = in[at_meta + i];
+                words[0] = in[at0 + (1 + kv) * i];  // lanes past the vector read what lies behind
+                words[1] = in[at1 + (1 + kv) * i];
+            } else {
+                const long long slot = __shfl_sync(FULL, t.slot, of8 + 8 * i);
                 if (left <= 8 * i) continue;
-                there = slot >= 0;
-                if (there) from = tile_at(pool, page_shift, slot, h, r);
+                if (slot >= 0) {
+                    int r;
+                    const uint32_t* from = tile_at(pool, page_shift, slot, h, r);
+                    meta = from[kv4_meta_word(nw, n, r, kv)];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (j < have) words[j] = from[kv ? kv4_v_word(nw, w + 4 * j, r) : kv4_k_word(nw, w + 4 * j, r)];
+                }
             }
-            const uint32_t meta = there ? from[kv4_meta_word(nw, n, r, kv)] : 0u;
             const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&meta));
-            const uint32_t* at = from + (kv ? kv4_v_word(nw, w, r) : kv4_k_word(nw, w, r));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if (j >= have) continue;
-                const uint32_t word = there ? at[j == 0 ? 0 : kv ? 16 : 2] : 0u;
+                const uint32_t word = words[j];
                 Raw<T> raw;
                 float x[8];
 #pragma unroll
@@ -307,7 +329,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_read_kernel(const Kv4Poo
                 }
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) raw.set2(e, x[e], x[e + 1]);
-                raw.template store<WIDE>(dst + 8 * i * step + 8 * j);
+                raw.template store<WIDE>(dst + 8 * i * step + 32 * j);
             }
         }
     };
@@ -327,7 +349,7 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_read_kernel(const Kv4Poo
 }
 
 bool wide_ok(const void* p, long long st, long long sh, int esize) {
-    return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(st * esize) | (uintptr_t)(sh * esize)) & 15);
+    return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(st * esize) | (uintptr_t)(sh * esize)) & (8 * esize - 1));
 }
 
 }  // namespace
