@@ -81,7 +81,7 @@ typedef struct {
                                 cache below; a quarter to a third of the fp16 bytes that every step
                                 reads).  As with fp16, the first decoder call reads the fp32 rows and
                                 every later one the stored ones.  At most 8 heads per K/V
-                                head; other calls (ms_generate, streams) keep kv_dtype */
+                                head, head sizes of multiples of 8 up to 64; other calls (ms_generate, streams) keep kv_dtype */
     int32_t reserved[5];
 } ms_options;
 
@@ -469,9 +469,12 @@ ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* tokens, int3
  * table's width, is not there.  With `causal`, query i of n sees only the positions up to
  * lens[b] - n + i (lens counts the queries' own positions); otherwise all.  Query head h reads
  * K/V head h / (heads / kv_heads).  out = softmax(scale q k^T) v, zeros for a query that sees
- * nothing; tokens of no row are left as they are.  Softmax and sums are fp32; the products take
+ * nothing; tokens of no row are left as they are.  A row's table spans at most 2^30 positions,
+ * and max_q * heads at most 65535 groups of 16 query rows of one K/V head (MS_F16 and MS_BF16
+ * prompts: of 128).  Softmax and sums are fp32; the products take
  * the codes exactly, q as fixed point of 16 bits (MS_F32: 24) relative to each (token, head)'s
- * largest value, and the probabilities as one fp16 value (MS_BF16) or two. */
+ * largest value (below 1e-30 it counts as zero), and the probabilities as one fp16 value
+ * (MS_BF16) or two. */
 typedef struct {
     const void* q;                                /* [q_tokens][heads][head_dim] */
     void* out;                                    /* the same shape; may not overlap q */

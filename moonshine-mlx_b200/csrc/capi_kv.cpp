@@ -1,5 +1,6 @@
 // extern "C" boundary of the 4-bit paged K/V cache operators: argument checks, the device, and
 // the launches (kernels/block_tables.cu, kv4_store.cu, kv4_attention.cu).
+#include <algorithm>
 #include <cmath>
 #include <exception>
 #include <string>
@@ -53,6 +54,11 @@ int elem_size(int32_t dtype) {
     return dtype == MS_F32 ? 4 : 2;
 }
 
+// rows of hd elements at these strides lie apart
+bool apart(int64_t tokens, int64_t heads, int64_t token_stride, int64_t head_stride, int hd) {
+    return (tokens <= 1 || token_stride >= hd) && (heads <= 1 || head_stride >= hd);
+}
+
 int type_of(int32_t dtype) { return dtype == MS_F32 ? KV4_F32 : dtype == MS_F16 ? KV4_F16 : KV4_BF16; }
 
 void check_tokens(const ms_kv4_tokens* t) {
@@ -103,7 +109,9 @@ Kv4Attention attention_of(const ms_kv4_pool* pool, const ms_kv4_attention_args* 
         need(a->block_table || a->width == 0, "null block_table");
         need(aligned(a->q, es) && aligned(a->out, es), "q and out must be aligned to their type");
         need(a->cu_q || a->q_tokens >= a->rows, "without cu_q q holds one token per row");
-        need((int64_t)a->width * pool->page_size < (int64_t)1 << 31, "a row's table spans 2^31 positions or more");
+        need((int64_t)a->width * pool->page_size <= (int64_t)1 << 30, "a row's table spans more than 2^30 positions");
+        need(apart(a->q_tokens, a->heads, a->out_token_stride, a->out_head_stride, pool->head_dim),
+             "out's strides are smaller than head_dim");
     }
     need(a->scale == a->scale && !std::isinf(a->scale), "scale must be finite");
     Kv4Attention k;
@@ -122,8 +130,10 @@ Kv4Attention attention_of(const ms_kv4_pool* pool, const ms_kv4_attention_args* 
     k.width = a->width;
     k.lens = a->lens;
     k.cu_q = a->cu_q;
-    k.max_q = a->cu_q ? a->max_q : 1;
+    k.max_q = a->cu_q ? (int)std::min<int64_t>(a->max_q, a->q_tokens) : 1;
     k.causal = a->causal != 0;
+    if (k.rows > 0 && k.max_q > 0 && !kv4_attention_fits(k, pool->kv_heads, pool->head_dim))
+        throw MsError(MS_ERR_UNSUPPORTED, "max_q * heads is too large: give the queries in several calls");
     k.scale = a->scale == 0.f ? (float)(1.0 / std::sqrt((double)pool->head_dim)) : a->scale;
     return k;
 }
@@ -176,6 +186,9 @@ ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* t, int32_t d
         const Kv4Pool p = pool_of(pool);
         check_tokens(t);
         if (t->tokens == 0) return;
+        need(apart(t->tokens, p.kv_heads, t->k_token_stride, t->k_head_stride, p.head_dim) &&
+                 apart(t->tokens, p.kv_heads, t->v_token_stride, t->v_head_stride, p.head_dim),
+             "strides of k or v are smaller than head_dim");
         DeviceScope d(device);
         MSB_CUDA(launch_kv4_read(p, t->k, t->v, type_of(t->dtype), t->tokens, t->k_token_stride, t->k_head_stride,
                                  t->v_token_stride, t->v_head_stride, reinterpret_cast<const long long*>(t->slots),

@@ -6,18 +6,28 @@
 namespace msb {
 namespace {
 
-AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
-    AttSplit sp;
-    // Rows per CTA: as many as one K/V head has, up to 16, or 128 in the wide kernel, whose stages
-    // take as long for 20 rows as for 128.  Against each other, 32 requests of 4000 positions, 4
+// Rows per CTA: as many as one K/V head has, up to 16, or 128 in the wide kernel.
+int rows_per_cta(const Kv4Attention& a, int kv_heads, int head_dim) {
+    // A stage of the wide kernel takes as long for 20 rows as for 128.  Against each other, 32 requests of 4000 positions, 4
     // K/V heads, bf16: heads of 64, 20 rows 61 (wide) and 59 us, 36 rows 74 and 82, 128 rows 90
     // and 158; heads of 128, 35 rows 133 and 123, 63 rows 141 and 168, 126 rows 162 and 246.
     // (fp32 has no wide kernel: its products need more planes.)
-    const long long rows = (long long)a.max_q * (a.heads / pool.kv_heads);
-    const bool wide = rows > 16 + 16 * kv4_groups(pool.head_dim) && (a.dtype == KV4_F16 || a.dtype == KV4_BF16);
-    sp.rows = wide ? 128 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-    const long long per_row = (rows + sp.rows - 1) / sp.rows * pool.kv_heads, pairs = per_row * a.rows;
-    sp.per_row = (int)std::min(per_row, (long long)INT_MAX);
+    const long long rows = (long long)a.max_q * (a.heads / kv_heads);
+    if (rows > 16 + 16 * kv4_groups(head_dim) && (a.dtype == KV4_F16 || a.dtype == KV4_BF16)) return 128;
+    return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+}
+// CTAs of one batch row
+long long ctas_per_row(const Kv4Attention& a, int kv_heads, int head_dim) {
+    const long long rows = (long long)a.max_q * (a.heads / kv_heads), each = rows_per_cta(a, kv_heads, head_dim);
+    return (rows + each - 1) / each * kv_heads;
+}
+
+AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
+    AttSplit sp;
+    sp.rows = rows_per_cta(a, pool.kv_heads, pool.head_dim);
+    const bool wide = sp.rows == 128;
+    const long long per_row = ctas_per_row(a, pool.kv_heads, pool.head_dim), pairs = per_row * a.rows;
+    sp.per_row = (int)per_row;
     const long long width = (long long)a.width * pool.page_size;
     // eight warps per CTA when there are fewer CTAs than half the GPU holds, two when there are
     // several waves of them (less to join and to wait for)
@@ -33,6 +43,12 @@ AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
     sp.chunk = few ? (width <= 1536 ? 1536 : 512) : pairs < slots ? 2048 : 4096;
     sp.splits = (int)std::max(1ll, (width + sp.chunk - 1) / sp.chunk);
     if (few) sp.splits = (int)std::min((long long)sp.splits, sp.ctas / per_row + 1);
+    // At most 256 MB of parts (prompts of thousands of tokens fill the GPU without them).
+    const long long each = a.q_tokens * a.heads * (pool.head_dim + 2) * 4, most = std::max(1ll, (256ll << 20) / each);
+    if (sp.splits > most) {
+        sp.splits = (int)most;
+        sp.chunk = (int)std::max((long long)sp.chunk, (width + most - 1) / most);
+    }
     const int tpp = pool.page_size / KV4_TILE;
     if ((tpp & (tpp - 1)) == 0)
         while (1 << (sp.page_shift + 1) <= tpp) ++sp.page_shift;
@@ -40,6 +56,10 @@ AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
 }
 
 }  // namespace
+
+bool kv4_attention_fits(const Kv4Attention& a, int kv_heads, int head_dim) {
+    return ctas_per_row(a, kv_heads, head_dim) <= 65535;
+}
 
 bool kv4_head_dim_ok(int hd) { return hd >= 8 && hd <= 128 && hd % 8 == 0; }
 
@@ -51,7 +71,6 @@ size_t kv4_attention_workspace(const Kv4Pool& pool, const Kv4Attention& a) {
 
 cudaError_t launch_kv4_attention(const Kv4Pool& pool, const Kv4Attention& a, void* workspace, cudaStream_t s) {
     AttSplit sp = split_of(pool, a);
-    if (sp.per_row > 65535) return cudaErrorInvalidConfiguration;
     sp.part = reinterpret_cast<float*>(workspace);
     if (sp.rows == 128) return launch_kv4_attention_wide(pool, a, sp, s);
     if (a.dtype == KV4_F32) return launch_kv4_attention_f32(pool, a, sp, s);

@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) kv4_attention_wide_kernel(con
     pdl_trigger();
     const uint32_t tmem = s_tmem;
     volatile int* failed = &s_failed;
+    int loaded = 0;  // stages that warp 9 asked for
 
     // Registers from the 3 x 80 of the launch: 136 for the softmax, 64 to unpack, 40 for the rest.
     if (wid >= 8) {
@@ -353,6 +354,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) kv4_attention_wide_kernel(con
                     bulk_load(smem_raw + (raw_at - smem_u32(smem_raw)) + slot * raw_bytes + lane * tile_bytes,
                               head + page * pool.page_stride + (long long)in_page * tile_bytes, len * tile_bytes,
                               &s_raw_full[slot]);
+                loaded = i + 1;
                 page = next;
                 in_page = in_next;
             }
@@ -625,6 +627,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) kv4_attention_wide_kernel(con
     fence_before();
     __syncthreads();
     fence_after();
+    if (wid == 9 && *failed)  // a role gave up: its copies in flight end before the CTA does
+        for (int i = max(0, loaded - WIDE_RAW); i < loaded; ++i) mbar_wait(&s_raw_full[i % WIDE_RAW], (i / WIDE_RAW) & 1);
     if (wid == 8)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(WIDE_COLS) : "memory");
 }

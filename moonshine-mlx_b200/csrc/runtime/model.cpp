@@ -533,8 +533,9 @@ Model* load_model(const std::string& dir, const ms_options& o) {
     m->num_sms = prop.multiProcessorCount;
     m->cfg = Config::from_json_file(dir + "/config.json");
     validate(m->cfg);
-    if (o.cross_kv_bits == 4 && m->cfg.heads / m->cfg.kv_heads > 8)
-        throw MsError(MS_ERR_UNSUPPORTED, "cross_kv_bits = 4 needs at most 8 heads per K/V head");
+    if (o.cross_kv_bits == 4 && (m->cfg.heads / m->cfg.kv_heads > 8 || m->cfg.head_dim > 64 || m->cfg.head_dim % 8))
+        throw MsError(MS_ERR_UNSUPPORTED,
+                      "cross_kv_bits = 4 needs at most 8 heads per K/V head, of a multiple of 8 up to 64");
     MSB_CUDA(cudaStreamCreateWithFlags(&m->stream, cudaStreamNonBlocking));
     for (auto& e : m->ev) MSB_CUDA(cudaEventCreate(&e));
 

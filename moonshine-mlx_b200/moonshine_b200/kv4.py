@@ -265,8 +265,8 @@ def kv4_attention(q, pool, block_table, lens, cu_q=None, max_q: Optional[int] = 
     code = a.codes.get(q.dtype)
     device = pool.get_device()
     shape, ps, qs, ts, tp = q.shape, pool.shape, q.stride(), block_table.shape, block_table.stride()
-    if scale is not None and not scale:
-        raise ValueError("scale must not be 0")
+    if scale is not None and not abs(scale) >= 1e-37:
+        raise ValueError(f"scale must be None or at least 1e-37 in magnitude, not {scale}")
     if cu_q is None:
         max_q = 1
     elif max_q is None:

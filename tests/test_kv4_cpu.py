@@ -84,10 +84,29 @@ def attention_struct(**changes):
     (dict(dtype=3), "dtype"), (dict(rows=-1), "negative"), (dict(heads=3), "multiple of kv_heads"),
     (dict(heads=0), "multiple of kv_heads"), (dict(q=None), "null q"), (dict(lens=None), "null q"),
     (dict(block_table=None), "null block_table"), (dict(rows=4), "one token per row"), (dict(q=(1 << 20) + 2), "aligned"),
-    (dict(scale=float("nan")), "finite"), (dict(width=1 << 28), "2^31"), (dict(rows=70000), "65535")])
+    (dict(scale=float("nan")), "finite"), (dict(width=(1 << 26) + 1), "2^30"), (dict(out_head_stride=63), "strides"), (dict(out_token_stride=0), "strides"), (dict(rows=70000), "65535")])
 def test_attention_refusals(changes, text):
     L, p = mb._L(), pool_struct()
     refused(L.ms_kv4_attention(p, attention_struct(**changes), None, 0, -1, None), text)
+
+
+def test_queries_that_do_not_fit_a_launch():
+    L, p = mb._L(), pool_struct()
+    many = dict(q_tokens=10 ** 6, max_q=10 ** 6, cu_q=1 << 20)
+    refused(L.ms_kv4_attention(p, attention_struct(**many), None, 0, -1, None), "several calls", UNSUPPORTED)
+    assert L.ms_kv4_attention_workspace(p, attention_struct(**many)) == -1
+    # max_q counts up to the tokens that there are; bf16 rows go 128 to a group
+    assert L.ms_kv4_attention_workspace(p, attention_struct(q_tokens=200, max_q=10 ** 9, cu_q=1 << 20)) == 0
+    assert L.ms_kv4_attention_workspace(p, attention_struct(dtype=2, **many)) == 0
+
+
+def test_workspace_is_bounded():
+    """Parts of long contexts take at most 256 MB, whatever the number of query tokens."""
+    L, p = mb._L(), pool_struct(page_size=64, page_stride=2 * 64 * 72, head_stride=64 * 72)
+    for tokens in (1, 100, 5000, 10 ** 5):
+        n = L.ms_kv4_attention_workspace(p, attention_struct(dtype=2, q_tokens=tokens, max_q=tokens, cu_q=1 << 20, rows=2,
+                                                             width=1 << 14))
+        assert 0 <= n <= 256 << 20, (tokens, n)
 
 
 def test_empty_calls_do_nothing():
@@ -108,6 +127,8 @@ def test_store_refusals(changes, text):
     refused(L.ms_kv4_append(p, tokens_struct(**changes), -1, None), text)
     refused(L.ms_kv4_read(p, tokens_struct(**changes), -1, None), text)
     refused(L.ms_kv4_append(None, tokens_struct(), -1, None), "null pool")
+    refused(L.ms_kv4_read(p, tokens_struct(k_head_stride=32), -1, None), "strides")
+    refused(L.ms_kv4_read(p, tokens_struct(v_token_stride=0), -1, None), "strides")
     refused(L.ms_kv4_append(p, None, -1, None), "null tokens")
 
 
@@ -144,6 +165,9 @@ def test_python_refusals():
         mb.kv_block_tables(i32(3), i32(3), i64(3, 4), 16, 5, n_pages=4)
     with pytest.raises(ValueError, match="page_size"):
         mb.kv4_pool(4, 2, 64, 24)
+    for scale in (0, 1e-60, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            mb.kv4_attention(torch.zeros(3, 4, 64), pool, i32(3, 4), i32(3), scale=scale)
 
 
 def test_structs_have_the_library_layout():

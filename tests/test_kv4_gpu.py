@@ -204,17 +204,20 @@ def build(lens, heads, hd, page, g, extra=2, fill=0xFF):
 
 
 def tolerance(out, mass, peak, dtype, hd):
-    """Half a step of the type for the result, and the roundings before it.  A score sums hd
+    """Half a step of the type for the result (below the smallest normal n all numbers are
+    multiples of n eps, so never less than n eps / 2: 2^-25 in fp16), and the roundings before
+    it.  A score sums hd
     products and the bias terms in fp32 (each addition 2^-23, tensor cores cut instead of
     rounding) over terms of `mass` in all -- s c and b are each up to twice a key's range, so
     4 mass -- plus fp32's q planes (2^-22); a wrong score shifts a probability, and so the
     result, by twice that times the largest value.  Probabilities in one fp16 plane are off by
     2^-12, in two by 2^-22, of terms s c up to twice the largest value; exp and the fp32 sums
     by 2^-20."""
-    half = torch.finfo(dtype).eps / 2
+    info = torch.finfo(dtype)
+    half = info.eps / 2
     score = 4 * mass * ((hd + 16) * 2.0 ** -23 + 2.0 ** -22)
     plane = 2.0 ** -12 if dtype == torch.bfloat16 else 2.0 ** -22
-    return out.abs() * half + (peak * (2 * score + 2 * plane + 2.0 ** -20)).unsqueeze(-1) + 1e-30
+    return out.abs().clamp(min=info.smallest_normal) * half + (peak * (2 * score + 2 * plane + 2.0 ** -20)).unsqueeze(-1) + 1e-30
 
 
 def check(got, want, mass, peak, dtype, hd):
@@ -471,3 +474,162 @@ def test_two_streams_at_once():
                 got.append(mb.kv4_attention(q, pool, table, n))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got)
+
+
+# ---------------------------------------------------------------- many query rows per K/V head
+# (heads, kv_heads, hd): one and two groups of 64, whole and partial
+MANY = [(8, 2, 40), (4, 4, 64), (5, 1, 80), (14, 2, 128)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,hd", MANY)
+def test_many_queries_missing_pages_and_queries_before_the_first_position(heads, kv_heads, hd, kind):
+    g = torch.Generator(device="cuda").manual_seed(hd + heads)
+    lens, qs, page = [333, 64, 20, 0, 150], [70, 64, 75, 40, 33], 16
+    pool, table, keys, values = build(lens, kv_heads, hd, page, g)
+    table[0, 3], table[0, 20], table[1, :], table[4, 0:2] = -1, pool.shape[0], -7, pool.shape[0] + 5
+    present = [torch.ones(n, dtype=torch.bool, device="cuda") for n in lens]
+    present[0][48:64] = False
+    present[0][320:] = False
+    present[1][:] = False
+    present[4][:32] = False
+    cu = [0]
+    for n in qs:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1], heads, hd, generator=g, device="cuda").to(TYPES[kind])
+    for causal in (True, False):
+        out = mb.kv4_attention(q, pool, table, ints(lens), cu_q=ints(cu), max_q=max(qs), causal=causal)
+        want, mass, peak = ref.attention(q, keys, values, lens, cu, causal, hd ** -0.5, present)
+        check(out, want, mass, peak, TYPES[kind], hd)
+        assert not out[cu[1]:cu[2]].any() and not out[cu[3]:cu[4]].any()
+        if causal:
+            assert not out[cu[2]:cu[2] + 55].any()  # 75 queries of 20 positions
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads,kv_heads,hd,context", [(8, 2, 64, 30011), (16, 4, 128, 9000), (9, 1, 24, 5000)])
+def test_many_queries_split_context(heads, kv_heads, hd, context, kind):
+    g = torch.Generator(device="cuda").manual_seed(context)
+    lens, qs = [context, 40], [64, 17]
+    pool, table, keys, values = build(lens, kv_heads, hd, 64, g)
+    q = torch.randn(81, heads, hd, generator=g, device="cuda").to(TYPES[kind])
+    args = dict(cu_q=ints([0, 64, 81]), max_q=64)
+    out = mb.kv4_attention(q, pool, table, ints(lens), **args)
+    want, mass, peak = ref.attention(q, keys, values, lens, [0, 64, 81], True, hd ** -0.5)
+    check(out, want, mass, peak, TYPES[kind], hd)
+    assert torch.equal(out, mb.kv4_attention(q, pool, table, ints(lens), **args))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd", [64, 96])
+def test_many_queries_nan_reaches_only_what_sees_it(hd, kind):
+    g = torch.Generator(device="cuda").manual_seed(17)
+    n, qn = 200, 150
+    k, v = random_kv(n, 2, hd, torch.float32, g)
+    v[100, 1, 5], k[180, 0, 3] = math.nan, math.nan
+    pool = mb.kv4_pool(13, 2, hd, 16)
+    mb.kv4_append(pool, k, v, torch.arange(n, device="cuda"))
+    table = torch.arange(13, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn(qn, 2, hd, generator=g, device="cuda").to(TYPES[kind])
+    q[7, 0, 2] = math.inf
+    out = mb.kv4_attention(q, pool, table, ints([n]), cu_q=ints([0, qn]), max_q=qn)
+    at = torch.arange(qn, device="cuda")
+    last = at + n - qn
+    # a NaN value makes its group of 64 dims NaN, a NaN key or query the whole row
+    want = torch.zeros(qn, 2, hd, dtype=torch.bool, device="cuda")
+    want[:, 1, :64] = (last >= 100)[:, None]
+    want[:, 0] = ((last >= 180) | (at == 7))[:, None]
+    assert torch.equal(torch.isnan(out), want)
+
+
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 300.0])
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_many_queries_value_and_query_sizes(size, kind):
+    g = torch.Generator(device="cuda").manual_seed(18)
+    hd, n, qn = 64, 333, 60
+    k, v = random_kv(n, 2, hd, torch.float32, g)
+    pool = mb.kv4_pool(-(-n // 16), 2, hd, 16)
+    slots = torch.arange(n, device="cuda")
+    mb.kv4_append(pool, k, v * size, slots)
+    ks, vs = (x.double() for x in mb.kv4_read(pool, slots, hd))
+    table = torch.arange(-(-n // 16), dtype=torch.int32, device="cuda")[None]
+    small = max(size, 1e-3)  # fp16 queries of 1e-3 .. 300 and back
+    q = (torch.randn(qn, 4, hd, generator=g, device="cuda") / small).to(TYPES[kind])
+    for sign in (1, -1):
+        out = mb.kv4_attention(q, pool, table, ints([n]), cu_q=ints([0, qn]), max_q=qn, scale=sign * small * hd ** -0.5)
+        want, mass, peak = ref.attention(q, [ks], [vs], [n], [0, qn], True, sign * small * hd ** -0.5)
+        check(out, want, mass, peak, TYPES[kind], hd)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_many_queries_strides_and_max_q(kind):
+    """Unaligned strided q and out; queries past max_q and tokens of no row stay as they were."""
+    g = torch.Generator(device="cuda").manual_seed(19)
+    lens, cu, hd, heads = [90, 300], [1, 41, 121], 64, 4
+    pool, table, keys, values = build(lens, 2, hd, 16, g)
+    big = torch.randn(heads, 125, 2 * hd + 1, generator=g, device="cuda").to(TYPES[kind])
+    q = big.transpose(0, 1)[:, :, 1:hd + 1]
+    for max_q in (80, 50):
+        room = torch.full((heads, 125, hd + 3), 5.0, device="cuda", dtype=TYPES[kind])
+        out = room.transpose(0, 1)[:, :, 1:hd + 1]
+        mb.kv4_attention(q, pool, table, ints(lens), cu_q=ints(cu), max_q=max_q, out=out)
+        want, mass, peak = ref.attention(q, keys, values, lens, cu, True, hd ** -0.5)
+        done = torch.zeros(125, dtype=torch.bool, device="cuda")
+        done[1:41] = True
+        done[41:41 + max_q] = True
+        check(out[done], want[done], mass[done], peak[done], TYPES[kind], hd)
+        assert (out[~done] == 5.0).all() and (room[:, :, 0] == 5.0).all() and (room[:, :, hd + 1:] == 5.0).all()
+
+
+def test_first_call_is_a_captured_one():
+    """Nothing of the library has run on the device before the capture."""
+    code = """
+import torch, moonshine_b200 as mb
+n, hd = 9000, 64
+pool = mb.kv4_pool(n // 16 + 1, 2, hd, 16)
+k = torch.randn(n, 2, hd, device="cuda"); slots = torch.empty(n, dtype=torch.int64, device="cuda")
+table = torch.full((1, n // 16 + 1), -1, dtype=torch.int32, device="cuda")
+zero = torch.zeros(1, dtype=torch.int32, device="cuda"); many = torch.full((1,), n, dtype=torch.int32, device="cuda")
+cu = torch.tensor([0, 40], dtype=torch.int32, device="cuda")
+one, q = torch.randn(1, 8, hd, device="cuda"), torch.randn(40, 8, hd, device="cuda").bfloat16()
+def run():
+    s, _, _ = mb.kv_block_tables(zero, many, table, 16, n, n_pages=pool.shape[0])
+    mb.kv4_append(pool, k, k, s)
+    return mb.kv4_attention(one, pool, table, many), mb.kv4_attention(q, pool, table, many, cu_q=cu, max_q=40), *mb.kv4_read(pool, s, hd)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(mb.__file__)))
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_two_graphs_of_split_contexts():
+    """Two captured calls, each with its own workspace, replayed on two streams at once."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    lens, hd = [20000, 100], 64
+    pool, table, keys, values = build(lens, 2, hd, 64, g)
+    n, graphs, outs, want = ints(lens), [], [], []
+    for i in range(2):
+        q = torch.randn(2, 8, hd, generator=g, device="cuda")
+        want.append(mb.kv4_attention(q, pool, table, n))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(mb.kv4_attention(q, pool, table, n))
+        graphs.append((graph, q))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for st, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
