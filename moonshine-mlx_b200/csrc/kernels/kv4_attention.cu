@@ -8,12 +8,17 @@ namespace {
 
 // Rows per CTA: as many as one K/V head has, up to 16, or 128 in the wide kernel.
 int rows_per_cta(const Kv4Attention& a, int kv_heads, int head_dim) {
-    // A stage of the wide kernel takes as long for 20 rows as for 128.  Against each other, 32 requests of 4000 positions, 4
-    // K/V heads, bf16: heads of 64, 20 rows 61 (wide) and 59 us, 36 rows 74 and 82, 128 rows 90
-    // and 158; heads of 128, 35 rows 133 and 123, 63 rows 141 and 168, 126 rows 162 and 246.
-    // (fp32 has no wide kernel: its products need more planes.)
+    // A stage of the wide kernel takes as long for 20 rows as for 128.  Against the other, us for
+    // ragged requests of 4 K/V heads, (33 of 1000 .. 8000 positions; 64 of 190 .. 1500):
+    //   bf16, heads of 64   20 rows (75; 36) and (64; 37), 32 (79; 36) and (75; 39), 64 (87; 40) and (121; 68)
+    //   bf16, heads of 128  20 rows (117; 53) and (100; 52), 32 (121; 54) and (111; 57), 35 (109; 57) and (132; 74)
+    //   fp16, heads of 64   32 rows (95; 49) and (76; 43), 48 (107; 53) and (103; 57), 64 (116; 54) and (132; 72)
+    //   fp16, heads of 128  48 rows (217; 100) and (161; 75), 64 (253; 105) and (213; 103)
+    // (fp16 takes the codes exactly, so its softmax does more.  fp32 has no wide kernel: its
+    // products need more planes.)
     const long long rows = (long long)a.max_q * (a.heads / kv_heads);
-    if (rows > 16 + 16 * kv4_groups(head_dim) && (a.dtype == KV4_F16 || a.dtype == KV4_BF16)) return 128;
+    if (rows > 32 && a.dtype == KV4_BF16) return 128;
+    if (rows > 32 + 16 * kv4_groups(head_dim) && a.dtype == KV4_F16) return 128;
     return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
 }
 // CTAs of one batch row

@@ -696,71 +696,76 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     }
 }
 
-// Joins the CTAs of contexts longer than one chunk, in their order: eight warps of a CTA on
-// eight (token, head) rows, or all on one (WIDE) when there are many parts, each warp taking
-// every eighth; four parts are loaded at a time.
+// Joins the CTAs of contexts longer than one chunk, in their order: a (token, head) row has 16
+// lanes (32 for more than 64 dims) of four dims each, of one warp, or of all eight of a CTA
+// (WIDE) when there are many parts, each warp taking every eighth; four parts are loaded at a time.
 template <class T, bool WIDE>
-__global__ void __launch_bounds__(256) kv4_attention_join_kernel(const Kv4Pool pool, const Kv4Attention a,
-                                                                 const AttSplit sp) {
-    __shared__ float s_v[8][128], s_l[8];
+__global__ void __launch_bounds__(256, 4) kv4_attention_join_kernel(const Kv4Pool pool, const Kv4Attention a,
+                                                                    const AttSplit sp) {
+    __shared__ float4 s_v[8][32];
+    __shared__ float s_l[8][32];
     pdl_wait();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, hd = pool.head_dim;
+    const int lanes = hd <= 64 ? 16 : 32, sub = lane & (lanes - 1);
     const int per = over(a.heads, pool.kv_heads);
     const int chunk = chunk_of(pool, a, sp);
     const Row row(pool, a, blockIdx.y);
-    const int r = WIDE ? blockIdx.x : blockIdx.x * 8 + wid, qi = r / a.heads, h = r % a.heads;
-    if (qi >= min(row.n, a.max_q)) return;
+    const int r = (WIDE ? blockIdx.x : blockIdx.x * 8 + wid) * (32 / lanes) + lane / lanes, qi = r / a.heads, h = r % a.heads;
     // the CTAs that had this row went by their last row's end
     const int in_head = qi * per + h % per, of = min(row.n, a.max_q) * per;
     const int last = min(in_head / sp.rows * sp.rows + sp.rows, of) - 1;
-    const int n = splits_of(row.end(a, over(last, per)), chunk);
-    if (n == 1) return;
+    int n = qi < min(row.n, a.max_q) ? splits_of(row.end(a, over(last, per)), chunk) : 1;
+    if (n == 1) n = 0;  // nothing to join
+    const bool dims = 4 * sub < hd;
     const long long tok = row.q0 + (long long)qi, each = a.q_tokens * a.heads, at = tok * a.heads + h;
     const float2* ml = reinterpret_cast<const float2*>(sp.part + sp.splits * each * hd) + at;
-    const float* part = sp.part + at * hd;
+    const float* part = sp.part + at * hd + 4 * sub;
     float mx = -INFINITY;
-    for (int s = lane; s < n; s += 32) mx = fmaxf(mx, ml[s * each].x);
-    mx = warp_max(mx);
-    float v[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+    for (int s = sub; s < n; s += lanes) mx = fmaxf(mx, ml[s * each].x);
+    for (int o = lanes / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ls = 0.f;
     constexpr int STEP = WIDE ? 8 : 1;
     for (int s0 = WIDE ? wid : 0; s0 < n; s0 += 4 * STEP) {
         float2 x[4];
-        float y[4][4];
+        float4 y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int s = s0 + i * STEP;
             x[i] = s < n ? ml[s * each] : make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                y[i][k] = s < n && lane + 32 * k < hd ? part[s * each * hd + lane + 32 * k] : 0.f;
+            y[i] = s < n && dims ? *reinterpret_cast<const float4*>(part + s * each * hd) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (x[i].y == 0.f) continue;  // saw nothing
             const float fs = x[i].x == -INFINITY ? 0.f : ex2(x[i].x - mx);
             ls = fmaf(x[i].y, fs, ls);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = fmaf(y[i][k], fs, v[k]);
+            v.x = fmaf(y[i].x, fs, v.x);
+            v.y = fmaf(y[i].y, fs, v.y);
+            v.z = fmaf(y[i].z, fs, v.z);
+            v.w = fmaf(y[i].w, fs, v.w);
         }
     }
     if constexpr (WIDE) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s_v[wid][lane + 32 * k] = v[k];
-        if (lane == 0) s_l[wid] = ls;
+        s_v[wid][lane] = v;
+        s_l[wid][lane] = ls;
         __syncthreads();
         if (wid) return;
 #pragma unroll
         for (int w = 1; w < 8; ++w) {
-            ls += s_l[w];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] += s_v[w][lane + 32 * k];
+            const float4 z = s_v[w][lane];
+            ls += s_l[w][lane];
+            v.x += z.x;
+            v.y += z.y;
+            v.z += z.z;
+            v.w += z.w;
         }
     }
-    const float inv = ls == 0.f ? 0.f : 1.f / ls;
-    const long long out = tok * a.out_token_stride + h * a.out_head_stride;
+    if (n == 0 || !dims) return;
+    const float inv = ls == 0.f ? 0.f : 1.f / ls, z[4] = {v.x, v.y, v.z, v.w};
+    const long long out = tok * a.out_token_stride + h * a.out_head_stride + 4 * sub;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (lane + 32 * k < hd) put<T>(a, out + lane + 32 * k, ls != ls ? NAN : v[k] * inv);
+    for (int k = 0; k < 4; ++k) put<T>(a, out + k, ls != ls ? NAN : z[k] * inv);
 }
 
 template <class T>
@@ -768,12 +773,10 @@ cudaError_t launch_join(const Kv4Pool& pool, const Kv4Attention& a, const AttSpl
     ++launch_counter();
     const bool pdl = pdl_launches();
     pdl_launches() = true;  // the join waits for the parts in the kernel: its launch overlaps them
-    const long long each = (long long)a.max_q * a.heads;
-    const cudaError_t j =
-        sp.splits > 8 ? launch_kernel(kv4_attention_join_kernel<T, true>, dim3((unsigned)each, a.rows), dim3(256), 0, s,
-                                      pool, a, sp)
-                      : launch_kernel(kv4_attention_join_kernel<T, false>, dim3((unsigned)((each + 7) / 8), a.rows),
-                                      dim3(256), 0, s, pool, a, sp);
+    const bool wide = sp.splits > 8;
+    const long long each = (long long)a.max_q * a.heads, rows = (wide ? 1 : 8) * (pool.head_dim <= 64 ? 2 : 1);
+    const cudaError_t j = launch_kernel(wide ? kv4_attention_join_kernel<T, true> : kv4_attention_join_kernel<T, false>,
+                                        dim3((unsigned)((each + rows - 1) / rows), a.rows), dim3(256), 0, s, pool, a, sp);
     pdl_launches() = pdl;
     return j;
 }

@@ -212,11 +212,13 @@ def tolerance(out, mass, peak, dtype, hd):
     4 mass -- plus fp32's q planes (2^-22); a wrong score shifts a probability, and so the
     result, by twice that times the largest value.  Probabilities in one fp16 plane are off by
     2^-12, in two by 2^-22, of terms s c up to twice the largest value; exp and the fp32 sums
-    by 2^-20."""
+    by 2^-20.  bf16 may take keys and values rounded to fp16, 2^-12 of each."""
     info = torch.finfo(dtype)
     half = info.eps / 2
     score = 4 * mass * ((hd + 16) * 2.0 ** -23 + 2.0 ** -22)
     plane = 2.0 ** -12 if dtype == torch.bfloat16 else 2.0 ** -22
+    if dtype == torch.bfloat16:
+        score, plane = score + mass * 2.0 ** -12, plane + 2.0 ** -13
     return out.abs().clamp(min=info.smallest_normal) * half + (peak * (2 * score + 2 * plane + 2.0 ** -20)).unsqueeze(-1) + 1e-30
 
 
