@@ -132,7 +132,8 @@ Kv4Attention attention_of(const ms_kv4_pool* pool, const ms_kv4_attention_args* 
     k.cu_q = a->cu_q;
     k.max_q = a->cu_q ? (int)std::min<int64_t>(a->max_q, a->q_tokens) : 1;
     k.causal = a->causal != 0;
-    if (k.rows > 0 && k.max_q > 0 && !kv4_attention_fits(k, pool->kv_heads, pool->head_dim))
+    const int64_t q_rows = (int64_t)k.max_q * a->heads;
+    if (q_rows >= (int64_t)1 << 30 || q_rows / pool->kv_heads >= 1 << 24)
         throw MsError(MS_ERR_UNSUPPORTED, "max_q * heads is too large: give the queries in several calls");
     k.scale = a->scale == 0.f ? (float)(1.0 / std::sqrt((double)pool->head_dim)) : a->scale;
     return k;

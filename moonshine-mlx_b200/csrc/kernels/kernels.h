@@ -425,8 +425,6 @@ cudaError_t launch_kv4_read(const Kv4Pool& pool, void* k, void* v, int dtype, lo
                             long long k_token_stride, long long k_head_stride, long long v_token_stride,
                             long long v_head_stride, const long long* slots, cudaStream_t s);
 // Workspace bytes of launch_kv4_attention (by sizes alone, not by the lengths on the device).
-// whether the queries fit one launch
-bool kv4_attention_fits(const Kv4Attention& a, int kv_heads, int head_dim);
 size_t kv4_attention_workspace(const Kv4Pool& pool, const Kv4Attention& a);
 cudaError_t launch_kv4_attention(const Kv4Pool& pool, const Kv4Attention& a, void* workspace, cudaStream_t s);
 bool kv4_head_dim_ok(int hd);

@@ -21,17 +21,13 @@ int rows_per_cta(const Kv4Attention& a, int kv_heads, int head_dim) {
     if (rows > 32 + 16 * kv4_groups(head_dim) && a.dtype == KV4_F16) return 128;
     return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
 }
-// CTAs of one batch row
-long long ctas_per_row(const Kv4Attention& a, int kv_heads, int head_dim) {
-    const long long rows = (long long)a.max_q * (a.heads / kv_heads), each = rows_per_cta(a, kv_heads, head_dim);
-    return (rows + each - 1) / each * kv_heads;
-}
 
 AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
     AttSplit sp;
     sp.rows = rows_per_cta(a, pool.kv_heads, pool.head_dim);
     const bool wide = sp.rows == 128;
-    const long long per_row = ctas_per_row(a, pool.kv_heads, pool.head_dim), pairs = per_row * a.rows;
+    const long long rows = (long long)a.max_q * (a.heads / pool.kv_heads);
+    const long long per_row = (rows + sp.rows - 1) / sp.rows * pool.kv_heads, pairs = per_row * a.rows;
     sp.per_row = (int)per_row;
     const long long width = (long long)a.width * pool.page_size;
     // eight warps per CTA when there are fewer CTAs than half the GPU holds, two when there are
@@ -49,7 +45,8 @@ AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
     sp.splits = (int)std::max(1ll, (width + sp.chunk - 1) / sp.chunk);
     if (few) sp.splits = (int)std::min((long long)sp.splits, sp.ctas / per_row + 1);
     // At most 256 MB of parts (prompts of thousands of tokens fill the GPU without them).
-    const long long each = a.q_tokens * a.heads * (pool.head_dim + 2) * 4, most = std::max(1ll, (256ll << 20) / each);
+    const long long each = a.q_tokens * a.heads * (pool.head_dim + 2) * 4;
+    const long long most = std::min(65535ll, std::max(1ll, (256ll << 20) / each));
     if (sp.splits > most) {
         sp.splits = (int)most;
         sp.chunk = (int)std::max((long long)sp.chunk, (width + most - 1) / most);
@@ -61,10 +58,6 @@ AttSplit split_of(const Kv4Pool& pool, const Kv4Attention& a) {
 }
 
 }  // namespace
-
-bool kv4_attention_fits(const Kv4Attention& a, int kv_heads, int head_dim) {
-    return ctas_per_row(a, kv_heads, head_dim) <= 65535;
-}
 
 bool kv4_head_dim_ok(int hd) { return hd >= 8 && hd <= 128 && hd % 8 == 0; }
 

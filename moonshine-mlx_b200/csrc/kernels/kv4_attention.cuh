@@ -238,8 +238,11 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     __shared__ int s_end[ROWS], s_from[F32 ? ROWS : 1][NG][QP];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, W = sp.warps;
     const int hd = HD ? HD : pool.head_dim, nw = kv4_words(hd), P = pool.page_size, per = over(a.heads, pool.kv_heads);
-    const int b = blockIdx.z, above = gridDim.y == pool.kv_heads ? 0 : blockIdx.y / pool.kv_heads;
-    const int kvh = blockIdx.y - above * pool.kv_heads, row0 = above * ROWS;
+    // The parts are the grid's slowest dimension: CTAs of parts that a short row does not have come
+    // last.  Between the others they cost 3 to 4 us of a slot each (4 contexts of 82K positions, 8
+    // heads of 64: 60 us, now 48; 33 of 8K, 28 heads on 4 of 128, lose 119 -> 123).
+    const int b = blockIdx.y, part_nr = blockIdx.z, above = gridDim.x == pool.kv_heads ? 0 : blockIdx.x / pool.kv_heads;
+    const int kvh = blockIdx.x - above * pool.kv_heads, row0 = above * ROWS;
     const int tile_words = kv4_tile_words(hd), tpp = P / KV4_TILE;
     const uint32_t tile_bytes = (uint32_t)tile_words * 4;
     unsigned char* ring = smem + (size_t)wid * ATT_STAGES * SU * tile_bytes;
@@ -295,14 +298,14 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     const int rows = min(ROWS, min(row.n, a.max_q) * per - row0);  // this CTA's (token, head) rows
     const int end = rows > 0 ? row.end(a, over(row0 + rows - 1, per)) : 0, all_see = rows > 0 ? row.end(a, over(row0, per)) : 0;
     const int n_split = splits_of(end, chunk);
-    if (rows <= 0 || (int)blockIdx.x >= n_split) {
+    if (rows <= 0 || part_nr >= n_split) {
         for (int i = 0; i < early; ++i) mbar_wait(&s_bar[wid][i], 0);
         return;
     }
     // its pieces of equal size, in whole runs
     constexpr int RUN = SU * KV4_TILE;
     const int piece = n_split == 1 ? end : ((end + n_split - 1) / n_split + RUN - 1) / RUN * RUN;
-    const int first = min(end, (int)blockIdx.x * piece), last = min(end, first + piece);
+    const int first = min(end, part_nr * piece), last = min(end, first + piece);
     // this warp's runs of SU tiles: wid, wid + W, ... of the piece
     const int tile0 = first / KV4_TILE, tiles = (last - first + KV4_TILE - 1) / KV4_TILE;
     const int runs = (tiles + SU - 1) / SU;
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
             for (int k = 0; k < 2 * NG; ++k)
                 if (lane + 32 * k < hd) put<T>(a, out + lane + 32 * k, ls != ls ? NAN : v[k] * inv);
         } else {
-            const long long each = a.q_tokens * a.heads, at = blockIdx.x * each + tok * a.heads + h;
+            const long long each = a.q_tokens * a.heads, at = part_nr * each + tok * a.heads + h;
 #pragma unroll
             for (int k = 0; k < 2 * NG; ++k)
                 if (lane + 32 * k < hd) sp.part[at * hd + lane + 32 * k] = v[k];
@@ -705,74 +708,69 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 
 // Joins the CTAs of contexts longer than one chunk, in their order: a (token, head) row has 16
 // lanes (32 for more than 64 dims) of four dims each, of one warp, or of all eight of a CTA
-// (WIDE) when there are many parts, each warp taking every eighth; four parts are loaded at a time.
+// (WIDE) when there are many parts, each warp taking every eighth.  Four parts are loaded at a
+// time and added under a running maximum, so that up to four cost one memory latency.
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(256, 4) kv4_attention_join_kernel(const Kv4Pool pool, const Kv4Attention a,
                                                                     const AttSplit sp) {
     __shared__ float4 s_v[8][32];
-    __shared__ float s_l[8][32];
+    __shared__ float2 s_ml[8][32];
     pdl_wait();
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, hd = pool.head_dim;
-    const int lanes = hd <= 64 ? 16 : 32, sub = lane & (lanes - 1);
-    const int per = over(a.heads, pool.kv_heads);
     const int chunk = chunk_of(pool, a, sp);
     const Row row(pool, a, blockIdx.y);
-    const int r = (WIDE ? blockIdx.x : blockIdx.x * 8 + wid) * (32 / lanes) + lane / lanes, qi = r / a.heads, h = r % a.heads;
-    // the CTAs that had this row went by their last row's end
-    const int in_head = qi * per + h % per, of = min(row.n, a.max_q) * per;
-    const int last = min(in_head / sp.rows * sp.rows + sp.rows, of) - 1;
-    int n = qi < min(row.n, a.max_q) ? splits_of(row.end(a, over(last, per)), chunk) : 1;
-    if (n == 1) n = 0;  // nothing to join
+    if (row.len <= chunk) return;  // nothing to join
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, hd = pool.head_dim;
+    const int lanes = hd <= 64 ? 16 : 32, sub = lane & (lanes - 1), at_once = (WIDE ? 1 : 8) * (32 / lanes);
+    const int per = over(a.heads, pool.kv_heads), tokens = min(row.n, a.max_q);
     const bool dims = 4 * sub < hd;
-    const long long tok = row.q0 + (long long)qi, each = a.q_tokens * a.heads, at = tok * a.heads + h;
-    const float2* ml = reinterpret_cast<const float2*>(sp.part + sp.splits * each * hd) + at;
-    const float* part = sp.part + at * hd + 4 * sub;
-    float mx = -INFINITY;
-    for (int s = sub; s < n; s += lanes) mx = fmaxf(mx, ml[s * each].x);
-    for (int o = lanes / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    float ls = 0.f;
-    constexpr int STEP = WIDE ? 8 : 1;
-    for (int s0 = WIDE ? wid : 0; s0 < n; s0 += 4 * STEP) {
-        float2 x[4];
-        float4 y[4];
+    const long long each = a.q_tokens * a.heads;
+    for (int r0 = blockIdx.x * at_once; r0 < tokens * a.heads; r0 += gridDim.x * at_once) {
+        const int r = r0 + (WIDE ? 0 : wid * (32 / lanes)) + lane / lanes, qi = r / a.heads, h = r - qi * a.heads;
+        // the CTAs that had this row went by their last row's end
+        const int in_head = qi * per + h % per;
+        const int last = min(in_head / sp.rows * sp.rows + sp.rows, tokens * per) - 1;
+        int n = qi < tokens ? splits_of(row.end(a, over(last, per)), chunk) : 1;
+        if (n == 1) n = 0;
+        const long long tok = row.q0 + (long long)qi, at = tok * a.heads + h;
+        const float2* ml = reinterpret_cast<const float2*>(sp.part + sp.splits * each * hd) + at;
+        const float* part = sp.part + at * hd + 4 * sub;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float mx = -INFINITY, ls = 0.f;
+        auto add = [&](float2 x, float4 y) {  // a part (maximum, sum) and its values; the sum of one that saw nothing is 0
+            if (x.y == 0.f) return;
+            const float now = fmaxf(mx, x.x), was = mx == -INFINITY ? 0.f : ex2(mx - now);
+            const float f = x.x == -INFINITY ? 0.f : ex2(x.x - now);
+            mx = now;
+            ls = fmaf(ls, was, x.y * f);
+            v = make_float4(fmaf(v.x, was, y.x * f), fmaf(v.y, was, y.y * f), fmaf(v.z, was, y.z * f), fmaf(v.w, was, y.w * f));
+        };
+        constexpr int STEP = WIDE ? 8 : 1;
+        for (int s0 = WIDE ? wid : 0; s0 < n; s0 += 4 * STEP) {
+            float2 x[4];
+            float4 y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = s0 + i * STEP;
-            x[i] = s < n ? ml[s * each] : make_float2(-INFINITY, 0.f);
-            y[i] = s < n && dims ? *reinterpret_cast<const float4*>(part + s * each * hd) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+            for (int i = 0; i < 4; ++i) {
+                const int s = s0 + i * STEP;
+                x[i] = s < n ? ml[s * each] : make_float2(-INFINITY, 0.f);
+                y[i] = s < n && dims ? *reinterpret_cast<const float4*>(part + s * each * hd) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (x[i].y == 0.f) continue;  // saw nothing
-            const float fs = x[i].x == -INFINITY ? 0.f : ex2(x[i].x - mx);
-            ls = fmaf(x[i].y, fs, ls);
-            v.x = fmaf(y[i].x, fs, v.x);
-            v.y = fmaf(y[i].y, fs, v.y);
-            v.z = fmaf(y[i].z, fs, v.z);
-            v.w = fmaf(y[i].w, fs, v.w);
+            for (int i = 0; i < 4; ++i) add(x[i], y[i]);
         }
+        if constexpr (WIDE) {
+            s_v[wid][lane] = v;
+            s_ml[wid][lane] = make_float2(mx, ls);
+            __syncthreads();
+            if (wid == 0)
+                for (int w = 1; w < 8; ++w) add(s_ml[w][lane], s_v[w][lane]);
+            __syncthreads();
+        }
+        if (n == 0 || !dims || (WIDE && wid != 0)) continue;
+        const float inv = ls == 0.f ? 0.f : 1.f / ls, z[4] = {v.x, v.y, v.z, v.w};
+        const long long out = tok * a.out_token_stride + h * a.out_head_stride + 4 * sub;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) put<T>(a, out + k, ls != ls ? NAN : z[k] * inv);
     }
-    if constexpr (WIDE) {
-        s_v[wid][lane] = v;
-        s_l[wid][lane] = ls;
-        __syncthreads();
-        if (wid) return;
-#pragma unroll
-        for (int w = 1; w < 8; ++w) {
-            const float4 z = s_v[w][lane];
-            ls += s_l[w][lane];
-            v.x += z.x;
-            v.y += z.y;
-            v.z += z.z;
-            v.w += z.w;
-        }
-    }
-    if (n == 0 || !dims) return;
-    const float inv = ls == 0.f ? 0.f : 1.f / ls, z[4] = {v.x, v.y, v.z, v.w};
-    const long long out = tok * a.out_token_stride + h * a.out_head_stride + 4 * sub;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) put<T>(a, out + k, ls != ls ? NAN : z[k] * inv);
 }
 
 template <class T>
@@ -781,9 +779,11 @@ cudaError_t launch_join(const Kv4Pool& pool, const Kv4Attention& a, const AttSpl
     const bool pdl = pdl_launches();
     pdl_launches() = true;  // the join waits for the parts in the kernel: its launch overlaps them
     const bool wide = sp.splits > 8;
-    const long long each = (long long)a.max_q * a.heads, rows = (wide ? 1 : 8) * (pool.head_dim <= 64 ? 2 : 1);
+    const long long at_once = (wide ? 1 : 8) * (pool.head_dim <= 64 ? 2 : 1);
+    // few CTAs per row of the batch when there are many: most rows may have nothing to join
+    const long long all = ((long long)a.max_q * a.heads + at_once - 1) / at_once, some = std::max(16, 148 * 8 / a.rows);
     const cudaError_t j = launch_kernel(wide ? kv4_attention_join_kernel<T, true> : kv4_attention_join_kernel<T, false>,
-                                        dim3((unsigned)((each + rows - 1) / rows), a.rows), dim3(256), 0, s, pool, a, sp);
+                                        dim3((unsigned)std::min(all, some), a.rows), dim3(256), 0, s, pool, a, sp);
     pdl_launches() = pdl;
     return j;
 }
@@ -799,7 +799,7 @@ cudaError_t launch_shape(const Kv4Pool& pool, const Kv4Attention& a, const AttSp
         if (e != cudaSuccess) return e;
     }
     ++launch_counter();
-    return launch_kernel(fn, dim3(sp.splits, sp.per_row, a.rows), dim3(32 * sp.warps), smem, s, pool, a, sp,
+    return launch_kernel(fn, dim3(sp.per_row, a.rows, sp.splits), dim3(32 * sp.warps), smem, s, pool, a, sp,
                          (int)S::ring(pool.head_dim, sp.warps));
 }
 

@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
     __shared__ __align__(8) uint64_t s_raw_full[RAW], s_raw_empty[RAW], s_raw_q, s_q;
     // Stage i has entry i % 4: K and V unpacked, S summed (and K unpacked, with what the softmax
     // reads of it), P written, O summed; what the softmax reads, i % 8.  K of stage i + 4 is
-    // unpacked after the scores of stage i + 1 are summed, V after the second product of stage
+    // unpacked after the softmax of stage i or a later one, V after the second product of stage
     // i + 1, so an entry's next phase waits, through the other roles, for whoever still has to
     // see this one.
     __shared__ __align__(8) uint64_t s_k[4], s_v[4], s_s[4], s_p[4], s_pv[4];
@@ -232,7 +232,8 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     const int hd = pool.head_dim, nw = kv4_words(hd), P = pool.page_size, per = over(a.heads, pool.kv_heads);
     // the last queries first: under a causal mask they see the most
-    const int b = blockIdx.z, y = gridDim.y - 1 - blockIdx.y, above = gridDim.y == pool.kv_heads ? 0 : y / pool.kv_heads;
+    const int b = blockIdx.y, part_nr = blockIdx.z, y = gridDim.x - 1 - blockIdx.x;
+    const int above = gridDim.x == pool.kv_heads ? 0 : y / pool.kv_heads;
     const int kvh = y - above * pool.kv_heads, row0 = above * WIDE_ROWS;
     pdl_wait();
     const int chunk = chunk_of(pool, a, sp);
@@ -241,9 +242,9 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
     if (rows <= 0) return;
     const int end = row.end(a, over(row0 + rows - 1, per)), all_see = row.end(a, over(row0, per));
     const int n_split = splits_of(end, chunk);
-    if ((int)blockIdx.x >= n_split) return;
+    if (part_nr >= n_split) return;
     const int piece = n_split == 1 ? end : ((end + n_split - 1) / n_split + WIDE_STEP - 1) / WIDE_STEP * WIDE_STEP;
-    const int first = min(end, (int)blockIdx.x * piece), last = min(end, first + piece);
+    const int first = min(end, part_nr * piece), last = min(end, first + piece);
     const int tile0 = first / KV4_TILE, tiles = (last - first + KV4_TILE - 1) / KV4_TILE;
     const int steps = (tiles + WIDE_TILES - 1) / WIDE_TILES;
     const int active = (rows + 31) / 32;  // softmax warps with rows
@@ -416,9 +417,12 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
             const int slot = i % RAW, i4 = i & 3, i8 = i & 7;
             if (!wait_on(&s_raw_full[slot], (i / RAW) & 1, failed)) break;
             // K's buffer is free when the scores of stage i - NK are summed, V's when its second
-            // product is; the scales' when the softmax of stage i - 2 has read them.
+            // product is; the scales' when the softmax of stage i - 2 has read them.  A group that
+            // unpacks every other stage has not seen stage i - 4 through: its entries are free
+            // when that softmax is done.
             if (i >= NK && !wait_on(&s_s[(i - NK) & 3], ((i - NK) >> 2) & 1, failed)) break;
             if (!ROUND && i >= 2 && !wait_on(&s_p[(i - 2) & 3], ((i - 2) >> 2) & 1, failed)) break;
+            if (EVERY > 1 && i >= 4 && !wait_on(&s_p[i4], ((i - 4) >> 2) & 1, failed)) break;
             const uint32_t k_to = k_buf + i % NK * NG * S::BLOCK, v_to = v_buf + i % NV * NG * S::BLOCK;
             const uint32_t okr = s_okr[slot];
             const bool here = (okr >> u) & 1;
@@ -746,7 +750,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
         const float l = good ? l2.x + l2.y : NAN;
         const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
         const bool done = n_split == 1;
-        const long long each = a.q_tokens * a.heads, at = blockIdx.x * each + tok * a.heads + h;
+        const long long each = a.q_tokens * a.heads, at = part_nr * each + tok * a.heads + h;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             float x[64];
@@ -801,7 +805,7 @@ cudaError_t launch_wide(const Kv4Pool& pool, const Kv4Attention& a, const AttSpl
                                          (int)smem);
     if (e != cudaSuccess) return e;
     ++launch_counter();
-    e = launch_kernel(fn, dim3(sp.splits, sp.per_row, a.rows), dim3(WideSmem<NG, is_bf16<T>>::THREADS), smem, s, pool, a, sp);
+    e = launch_kernel(fn, dim3(sp.per_row, a.rows, sp.splits), dim3(WideSmem<NG, is_bf16<T>>::THREADS), smem, s, pool, a, sp);
     return e != cudaSuccess || sp.splits == 1 ? e : launch_join<T>(pool, a, sp, s);
 }
 

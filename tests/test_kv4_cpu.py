@@ -92,12 +92,12 @@ def test_attention_refusals(changes, text):
 
 def test_queries_that_do_not_fit_a_launch():
     L, p = mb._L(), pool_struct()
-    many = dict(q_tokens=10 ** 6, max_q=10 ** 6, cu_q=1 << 20)
+    many = dict(q_tokens=10 ** 7, max_q=10 ** 7, cu_q=1 << 20)
     refused(L.ms_kv4_attention(p, attention_struct(**many), None, 0, -1, None), "several calls", UNSUPPORTED)
     assert L.ms_kv4_attention_workspace(p, attention_struct(**many)) == -1
-    # max_q counts up to the tokens that there are; bf16 rows go 128 to a group
+    # max_q counts up to the tokens that there are
     assert L.ms_kv4_attention_workspace(p, attention_struct(q_tokens=200, max_q=10 ** 9, cu_q=1 << 20)) == 0
-    assert L.ms_kv4_attention_workspace(p, attention_struct(dtype=2, **many)) == 0
+    assert L.ms_kv4_attention_workspace(p, attention_struct(q_tokens=10 ** 6, max_q=10 ** 6, cu_q=1 << 20)) == 0
 
 
 def test_workspace_is_bounded():

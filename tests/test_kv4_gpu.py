@@ -635,3 +635,15 @@ def test_two_graphs_of_split_contexts():
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_many_query_rows_of_a_long_prompt():
+    """More groups of query rows than a grid's second dimension holds."""
+    g = torch.Generator(device="cuda").manual_seed(32)
+    n, heads, hd = 140000, 8, 8
+    pool, table, keys, values = build([20], 8, hd, 16, g)
+    q = torch.randn(n, heads, hd, generator=g, device="cuda")
+    out = mb.kv4_attention(q, pool, table, ints([20]), cu_q=ints([0, n]), max_q=n, causal=False)
+    some = torch.cat([torch.arange(50, device="cuda"), torch.arange(n - 50, n, device="cuda")])
+    want, mass, peak = ref.attention(q[some], keys, values, [20], [0, 100], False, hd ** -0.5)
+    check(out[some], want, mass, peak, torch.float32, hd)
