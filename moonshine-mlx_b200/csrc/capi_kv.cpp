@@ -107,6 +107,7 @@ Kv4Attention attention_of(const ms_kv4_pool* pool, const ms_kv4_attention_args* 
     if (a->rows > 0 && a->q_tokens > 0 && a->max_q > 0) {
         need(a->q && a->out && a->lens, "null q, out or lens");
         need(a->block_table || a->width == 0, "null block_table");
+        need(a->q != a->out, "out may not be q");
         need(aligned(a->q, es) && aligned(a->out, es), "q and out must be aligned to their type");
         need(a->cu_q || a->q_tokens >= a->rows, "without cu_q q holds one token per row");
         need((int64_t)a->width * pool->page_size <= (int64_t)1 << 30, "a row's table spans more than 2^30 positions");

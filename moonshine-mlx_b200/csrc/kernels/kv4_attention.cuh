@@ -27,7 +27,7 @@
 // Bound: issue inside a run (60 to 80 % of the slots), and 4 to 6 us of latency per CTA around
 // them (2560 CTAs of one position take 16 us).  bf16, at the cache's bytes: 256 contexts of 187 ..
 // 1500 on 10 heads of 64, 50 us (3.2 TB/s, half of copy bandwidth); four of 16K .. 131K on 32 heads
-// of 128, 4 per K/V head, 91 us (4.1 TB/s, 64 %); one of 1500 in fp32, 10 us.
+// of 128, 4 per K/V head, 86 to 89 us (4.3 TB/s, 66 %); one of 1500 in fp32, 10 us.
 #pragma once
 
 #include <climits>

@@ -25,8 +25,8 @@
 // Two CTAs share an SM.  Bound: latency inside the roles; of a stage's 1300 cycles (64 dims, bf16)
 // the 64 exponentials of a warp are 512, and the tensor pipe is active 14 % of the time.  Measured,
 // 592 CTAs of 2048 positions: bf16 103 us (64 dims), 156 us (128); fp16 155 and 288 us.  8 prompts of
-// up to 512 tokens over up to 4096 positions, 16 heads on 4: 82 us, of which the longest rows' CTAs,
-// which meet on some SMs, take all: cut into pieces of 2048 the parts cost more (96 us).
+// up to 512 tokens over up to 4096 positions, 16 heads on 4: 83 us, of which the longest rows' CTAs,
+// which meet on some SMs, take all: cut into pieces of 2048 the parts cost more (90 to 98 us).
 #define KV4_ATTENTION_KERNELS
 #include "kv4_attention.cuh"
 

@@ -84,7 +84,7 @@ def attention_struct(**changes):
     (dict(dtype=3), "dtype"), (dict(rows=-1), "negative"), (dict(heads=3), "multiple of kv_heads"),
     (dict(heads=0), "multiple of kv_heads"), (dict(q=None), "null q"), (dict(lens=None), "null q"),
     (dict(block_table=None), "null block_table"), (dict(rows=4), "one token per row"), (dict(q=(1 << 20) + 2), "aligned"),
-    (dict(scale=float("nan")), "finite"), (dict(width=(1 << 26) + 1), "2^30"), (dict(out_head_stride=63), "strides"), (dict(out_token_stride=0), "strides"), (dict(rows=70000), "65535")])
+    (dict(scale=float("nan")), "finite"), (dict(width=(1 << 26) + 1), "2^30"), (dict(out_head_stride=63), "strides"), (dict(out_token_stride=0), "strides"), (dict(out=1 << 20), "may not be q"), (dict(rows=70000), "65535")])
 def test_attention_refusals(changes, text):
     L, p = mb._L(), pool_struct()
     refused(L.ms_kv4_attention(p, attention_struct(**changes), None, 0, -1, None), text)
