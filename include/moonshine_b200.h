@@ -474,7 +474,7 @@ ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* tokens, int3
  * the codes exactly, q as fixed point of 16 bits (MS_F32: 24) relative to each (token, head)'s
  * largest value (below 1e-30 it counts as zero), and the probabilities as one fp16 value
  * (MS_BF16) or two.  With more than 32 query rows per K/V head MS_BF16 takes keys and values
- * rounded to fp16. */
+ * rounded to fp16 (held to +-65504). */
 typedef struct {
     const void* q;                                /* [q_tokens][heads][head_dim] */
     void* out;                                    /* the same shape; may not overlap q */

@@ -647,3 +647,45 @@ def test_many_query_rows_of_a_long_prompt():
     some = torch.cat([torch.arange(50, device="cuda"), torch.arange(n - 50, n, device="cuda")])
     want, mass, peak = ref.attention(q[some], keys, values, [20], [0, 100], False, hd ** -0.5)
     check(out[some], want, mass, peak, torch.float32, hd)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(6, 2, 64, 48), (8, 1, 128, 112), (3, 1, 8, 16), (16, 4, 72, 80)])
+def test_many_queries_page_sizes(heads, kv_heads, hd, page, kind):
+    """Pages that end inside a stage of 64 positions, and one that holds several."""
+    g = torch.Generator(device="cuda").manual_seed(page + hd)
+    lens, qs = [517, 48, 113], [65, 48, 80]
+    pool, table, keys, values = build(lens, kv_heads, hd, page, g)
+    cu = [0, 65, 113, 193]
+    q = torch.randn(193, heads, hd, generator=g, device="cuda").to(TYPES[kind])
+    out = mb.kv4_attention(q, pool, table, ints(lens), cu_q=ints(cu), max_q=80)
+    want, mass, peak = ref.attention(q, keys, values, lens, cu, True, hd ** -0.5)
+    check(out, want, mass, peak, TYPES[kind], hd)
+
+
+@pytest.mark.parametrize("queries", [1, 100])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_largest_values(kind, queries):
+    """Ranges up to +-65504, whose highest code can stand for more than fp16's largest: the scale,
+    up to 8736, is rounded by at most 4, 15 times that is 60, and the bias by at most 16, so for
+    at most 65580.  Where values are held to 65504, that is off by 76 / 65580 < 2^-9.7."""
+    g = torch.Generator(device="cuda").manual_seed(41)
+    hd, n = 64, 100
+    k, v = random_kv(n, 1, hd, torch.float32, g)
+    k, v = k * 2e4, v * 4e4
+    v[::3, :, 0], v[::3, :, 1] = 65504, -65504
+    k[5, 0, 7], k[5, 0, 8] = 65504, -65504
+    pool = mb.kv4_pool(7, 1, hd, 16)
+    slots = torch.arange(n, device="cuda")
+    mb.kv4_append(pool, k, v, slots)
+    ks, vs = (x.double() for x in mb.kv4_read(pool, slots, hd))
+    assert 65504 < vs.max() <= 65580
+    table = torch.arange(7, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn(queries, 1, hd, generator=g, device="cuda").to(TYPES[kind])
+    scale = 1e-4 * hd ** -0.5
+    out = mb.kv4_attention(q, pool, table, ints([n]), cu_q=ints([0, queries]), max_q=queries, scale=scale)
+    want, mass, peak = ref.attention(q, [ks], [vs], [n], [0, queries], True, scale)
+    # where K and V are rounded to fp16 the tolerance has 2^-12 of keys and 2 (2^-12 + 2^-13) of
+    # values; 2^-9.7 more is 2^2.3 < 5 times and 2^1.3 / 1.5 < 1.7 times that
+    held = kind == "bf16" and queries > 32
+    check(out, want, mass * (6 if held else 1), peak * (2.7 if held else 1), TYPES[kind], hd)
