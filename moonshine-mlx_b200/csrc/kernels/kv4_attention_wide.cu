@@ -754,6 +754,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             float x[64];
+            __syncwarp();  // lanes without a row left the group before early
             if (steps > 0) {
                 tmem_ld32(mine_at + O_COL + 64 * n, x);
                 tmem_ld32(mine_at + O_COL + 64 * n + 32, x + 32);
