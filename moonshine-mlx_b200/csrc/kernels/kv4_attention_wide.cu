@@ -180,19 +180,20 @@ __device__ __forceinline__ void values_of(uint32_t x, uint32_t s, uint32_t b, bo
 
 __device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-// Bounded wait that also ends when another role has given up.
+// Bounded wait of a warp that also ends when another role has given up.  Its lanes agree on how
+// it ended: what follows (votes, shuffles, tensor memory) wants all of them or none.
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* failed) {
     const uint32_t a = smem_u32(bar);
+    uint32_t ok = 0;
     for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
-        uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
             : "r"(a), "r"(parity)
             : "memory");
-        if (ok) return true;
-        if ((i & 255) == 255 && *failed) return false;
+        if (ok || ((i & 255) == 255 && *failed)) break;
     }
+    if (__all_sync(FULL, ok)) return true;
     *failed = 1;
     return false;
 }
@@ -746,7 +747,6 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
         }
         if (steps > 0 && good) good = wait_on(&s_pv[(steps - 1) & 3], ((steps - 1) >> 2) & 1, failed);
         fence_after();
-        good = __all_sync(FULL, good);
         const float l = good ? l2.x + l2.y : NAN;
         const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
         const bool done = n_split == 1;
