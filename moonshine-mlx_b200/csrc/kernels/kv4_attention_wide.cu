@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
     const uint32_t q_at = base, k_buf = q_at + S::Q, v_buf = k_buf + S::K, raw_at = v_buf + S::V;
     const int tile_words = kv4_tile_words(hd), tpp = P / KV4_TILE;
     const uint32_t tile_bytes = (uint32_t)tile_words * 4, raw_bytes = (WIDE_TILES * tile_bytes + 127) / 128 * 128;
-    int loaded = 0;  // stages that the load warp asked for
+    int loaded = 0, issued = 0;  // stages that the load warp asked for, and a product warp
     auto load = [&](int i) {  // lane v stands for tile v of stage i
         const int* table = a.table + (long long)b * a.table_stride;
         const char* head = reinterpret_cast<const char*>(pool.base) + kvh * pool.head_stride;
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
             const bool there = wait_on(&s_q, 0, failed);
             const uint64_t q_desc = sw128_desc(q_at), k_desc = sw128_desc(k_buf);
 #pragma unroll 1
-            for (int i = 0; there && i < steps; ++i) {
+            for (int i = 0; there && i < steps; issued = ++i) {
                 if (!wait_on(&s_k[i & 3], (i >> 2) & 1, failed)) break;
                 // P of stage i - NS lies where S goes
                 if (i >= NS && !wait_on(&s_pv[(i - NS) & 3], ((i - NS) >> 2) & 1, failed)) break;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
             // O; one P for all groups: one product over the dims of both
             const uint64_t v_desc = sw128_desc(v_buf);
 #pragma unroll 1
-            for (int i = 0; i < steps; ++i) {
+            for (int i = 0; i < steps; issued = ++i) {
                 if (!wait_on(&s_v[i & 3], (i >> 2) & 1, failed) || !wait_on(&s_p[i & 3], (i >> 2) & 1, failed)) break;
                 fence_after();
 #pragma unroll
@@ -792,8 +792,11 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
     fence_before();
     __syncthreads();
     fence_after();
-    if (wid == S::LAST + 1 && *failed)  // a role gave up: its copies in flight end before the CTA does
+    if (*failed) {  // a role gave up: what is in flight ends before its memory goes
         for (int i = max(0, loaded - RAW); i < loaded; ++i) mbar_wait(&s_raw_full[i % RAW], (i / RAW) & 1);
+        if (issued > 0) mbar_wait(wid == S::LAST ? &s_s[(issued - 1) & 3] : &s_pv[(issued - 1) & 3], ((issued - 1) >> 2) & 1);
+        __syncthreads();
+    }
     if (wid == S::LAST)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(WIDE_COLS) : "memory");
 }
