@@ -485,7 +485,8 @@ typedef struct {
     const int32_t* lens;                          /* [rows] */
     const int32_t* cu_q;                          /* nullable, [rows + 1] ascending */
     int32_t dtype, heads, rows, width;
-    int32_t max_q;                                /* at least every row's queries; those past it are left out */
+    int32_t max_q;                                /* at least every row's queries; those past it are left out
+                                                     (without cu_q it counts as 1) */
     int32_t causal;
     float scale;                                  /* 0: head_dim^-1/2 */
     int32_t reserved;

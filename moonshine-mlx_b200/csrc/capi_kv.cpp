@@ -104,7 +104,8 @@ Kv4Attention attention_of(const ms_kv4_pool* pool, const ms_kv4_attention_args* 
     need(a->heads > 0 && a->heads % pool->kv_heads == 0, "heads must be a positive multiple of kv_heads");
     need(a->rows <= 65535, "at most 65535 rows per call");
     need(a->heads <= 65535, "at most 65535 heads");
-    if (a->rows > 0 && a->q_tokens > 0 && a->max_q > 0) {
+    const int max_q = a->cu_q ? (int)std::min<int64_t>(a->max_q, a->q_tokens) : 1;
+    if (a->rows > 0 && a->q_tokens > 0 && max_q > 0) {
         need(a->q && a->out && a->lens, "null q, out or lens");
         need(a->block_table || a->width == 0, "null block_table");
         need(a->q != a->out, "out may not be q");
@@ -131,7 +132,7 @@ Kv4Attention attention_of(const ms_kv4_pool* pool, const ms_kv4_attention_args* 
     k.width = a->width;
     k.lens = a->lens;
     k.cu_q = a->cu_q;
-    k.max_q = a->cu_q ? (int)std::min<int64_t>(a->max_q, a->q_tokens) : 1;
+    k.max_q = max_q;
     k.causal = a->causal != 0;
     const int64_t q_rows = (int64_t)k.max_q * a->heads;
     if (q_rows >= (int64_t)1 << 30 || q_rows / pool->kv_heads >= 1 << 24)
