@@ -403,7 +403,8 @@ ms_status ms_generate_long(ms_model* model, const float* audio, int64_t n_sample
  * and pages that the device memory then holds.  Argument errors are found before anything
  * is enqueued.
  *
- * Pages.  A pool holds `pages` pages of page_size positions (a multiple of 16), each position
+ * Pages.  A pool holds `pages` pages of page_size positions (a multiple of 16, at most
+ * 2^30), each position
  * with kv_heads K and V vectors of head_dim values (a multiple of 8, at most 128).  A vector's
  * values are cut into groups of 64 (the last one shorter); a group is stored as 4-bit codes c,
  * an fp16 scale s and an fp16 bias b (the affine form of the quantized checkpoints) and

@@ -78,7 +78,8 @@ void check_head_dim(int32_t hd) {
 Kv4Pool pool_of(const ms_kv4_pool* p) {
     need(p != nullptr, "null pool");
     check_head_dim(p->head_dim);
-    need(p->page_size > 0 && p->page_size % 16 == 0, "page_size must be a positive multiple of 16");
+    need(p->page_size > 0 && p->page_size % 16 == 0 && p->page_size <= 1 << 30,
+         "page_size must be a positive multiple of 16, at most 2^30");
     need(p->pages >= 0 && p->kv_heads > 0, "pages must not be negative and kv_heads must be positive");
     need(p->base || p->pages == 0, "null pool base");
     need(aligned(p->base, 16) && p->page_stride % 16 == 0 && p->head_stride % 16 == 0,

@@ -19,3 +19,26 @@ def test_without_cu_q_max_q_has_no_say(changes, text, max_q):
     assert L.ms_kv4_attention_workspace(p, args) == -1
     assert text in L.ms_last_error().decode()
     refused(L.ms_kv4_attention(p, args, None, 0, -1, None), text)
+
+
+def test_largest_page_size():
+    """Pages of more than 2^30 positions are refused (in a process of its own: the call once did
+    not return)."""
+    code = """
+import ctypes as C, moonshine_b200 as mb
+from moonshine_b200 import kv4
+L = mb._L()
+for page_size in (2 ** 30 + 16, 2 ** 31 - 16):
+    pool = C.byref(kv4._Kv4Pool(base=None, page_stride=0, head_stride=0, pages=0, kv_heads=1, head_dim=64, page_size=page_size))
+    t = C.byref(kv4._Kv4Tokens(k=1 << 20, v=1 << 21, slots=1 << 20, tokens=3, k_token_stride=64, k_head_stride=64,
+                               v_token_stride=64, v_head_stride=64, dtype=0, reserved=0))
+    for call in (L.ms_kv4_append, L.ms_kv4_read):
+        assert call(pool, t, -1, None) == 1 and b"page_size" in L.ms_last_error()
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(mb.__file__)))
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True,
+                       timeout=60)
+    assert r.returncode == 0, r.stderr[-2000:]
