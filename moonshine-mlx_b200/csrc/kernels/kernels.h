@@ -412,6 +412,7 @@ struct Kv4Attention {
     int max_q = 1, causal = 0;
     float scale = 1.f;
     size_t lo_off = 0;  // KV4_STEP: elements from the high plane to the low one, 0: none
+    unsigned* status = nullptr;  // up to 32 query rows per K/V head: DEV_WAIT_TIMEOUT when a wait ran out (null: only NaNs)
 };
 cudaError_t launch_block_tables(const int* lengths, const int* added, int rows, int page, const int* free_pages,
                                 int n_free, int* table, int width, long long table_stride, long long* slots,

@@ -56,6 +56,9 @@ cudaError_t launch_kv4_attention_wide(const Kv4Pool& pool, const Kv4Attention& a
 cudaError_t launch_kv4_attention_step(const Kv4Pool& pool, const Kv4Attention& a, const AttSplit& sp, cudaStream_t s);
 
 #ifdef KV4_ATTENTION_KERNELS
+#ifndef KV4_WAIT_LIMIT  // polls of a wait for a copy; a test has it run out
+#define KV4_WAIT_LIMIT WAIT_LIMIT
+#endif
 namespace {
 
 constexpr int ATT_WARPS = 8;   // most per CTA
@@ -622,15 +625,10 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         }
     };
     const int see = min(all_see, last) / KV4_TILE - tile0;  // whole tiles that every query sees
-    int slot = 0;
+    int slot = 0, run = wid;
     uint32_t phase = 0;
-    for (int run = wid; run < runs; run += W) {
-        if (!mbar_wait(&s_bar[wid][slot], phase)) {  // never seen: no result rather than a wrong one
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) l[nt][c] = NAN;
-        }
+    for (; run < runs; run += W) {
+        if (!__all_sync(FULL, mbar_wait(&s_bar[wid][slot], phase, KV4_WAIT_LIMIT))) break;
         const uint32_t ok = s_ok[wid][slot];
         if (ok == (1u << SU) - 1 && (run + 1) * SU <= see) work(std::true_type{}, run, slot, ok);
         else work(std::false_type{}, run, slot, ok);
@@ -642,6 +640,15 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         }
     }
 
+    if (run < runs) {  // a copy did not come: no result rather than a wrong one, once no other is in flight
+        if (lane == 0 && a.status) atomicCAS(a.status, 0u, (unsigned)DEV_WAIT_TIMEOUT);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) l[nt][c] = NAN;
+        for (int i = 0; i < ATT_STAGES && run + i * W < runs; ++i)
+            mbar_wait(&s_bar[wid][(slot + i) % ATT_STAGES], phase ^ (uint32_t)((slot + i) / ATT_STAGES));
+    }
     for (int i = 0; i < early; ++i)
         if (wid + i * W >= runs) mbar_wait(&s_bar[wid][i], 0);
 

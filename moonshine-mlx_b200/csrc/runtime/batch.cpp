@@ -224,6 +224,7 @@ Kv4Attention BatchEngine::cross4_args(int B) const {
     a.lens = frames.as<int>();
     a.scale = std::pow((float)c.head_dim, -0.5f);
     a.lo_off = split ? (size_t)Bc * HD : 0;
+    a.status = status.as<unsigned>();
     return a;
 }
 
