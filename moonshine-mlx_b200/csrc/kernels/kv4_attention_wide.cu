@@ -451,12 +451,14 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
                         odd |= not_finite(vs[x][n]) ? 1u << (8 * n + g) : 0u;
-                        most = max(most, max(ks[x][n] & 0x7fffu, vs[x][n] & 0x7fffu));
+                        // what code 15 stands for, in the low half: the group's largest, monotone in c
+                        most = max(most, max(hfma2_of(ks[x][n], 0x4b80u, ks[x][n] >> 16) & 0x7fffu,
+                                             hfma2_of(vs[x][n], 0x4b80u, vs[x][n] >> 16) & 0x7fffu));
                     }
                     odd = __reduce_or_sync(FULL, odd);
                     if (lane == 0) s_odd[i8][4 * (half0 + x) + u] = odd;
                 }
-                huge = __any_sync(FULL, most >= 0x6c00u);  // a scale of 4096 or more: s c + b may pass fp16's largest
+                huge = __any_sync(FULL, most >= 0x7c00u);  // a value of the tile that fp16 does not hold
             } else {
 #pragma unroll
                 for (int x = 0; x < HALVES; ++x) {

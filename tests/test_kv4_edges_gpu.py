@@ -40,3 +40,35 @@ def test_a_wait_that_runs_out_is_reported(tmp_path):
                     os.path.join(here, "kv4_give_up.cu")], check=True, timeout=300)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.split() == ["5", "0"], (r.returncode, r.stdout)
+
+
+# ---------------------------------------------------------------- the end of fp16's range
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("queries", [1, 70])
+def test_largest_code_past_fp16(queries, kind, which):
+    """A group from 34108.25 to 65504: s = 2094, b = 34112, and its code 15 stands for 65522, fp16's
+    infinity.  Where bf16 takes keys and values as fp16 it is held to 65504, off by 18 / 65522 <
+    2^-11.8: of keys beside the 2^-12 that the tolerance has (2.2 times that), of values beside
+    2 (2^-12 + 2^-13) (1.4 times that).  Queries that do not see the position are as without it."""
+    g = torch.Generator(device="cuda").manual_seed(51)
+    hd, n = 64, 100
+    k, v = random_kv(n, 1, hd, torch.float32, g)
+    k, v = k * (1e3 if which == "k" else 1), v * (1e3 if which == "v" else 1)
+    (k if which == "k" else v)[80, 0] = torch.linspace(34108.25, 65504, hd, device="cuda")
+    pool = mb.kv4_pool(7, 1, hd, 16)
+    slots = torch.arange(n, device="cuda")
+    mb.kv4_append(pool, k, v, slots)
+    ks, vs = (x.double() for x in mb.kv4_read(pool, slots, hd))
+    assert (ks if which == "k" else vs)[80].max() == 34112 + 15 * 2094
+    table = torch.arange(7, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn(queries, 1, hd, generator=g, device="cuda").to(TYPES[kind])
+    scale = hd ** -0.5 * (1e-4 if which == "k" else 1)
+    out = mb.kv4_attention(q, pool, table, ints([n]), cu_q=ints([0, queries]), max_q=queries, scale=scale)
+    want, mass, peak = ref.attention(q, [ks], [vs], [n], [0, queries], True, scale)
+    if kind == "fp16":  # results past fp16's largest are infinite
+        want = want.to(torch.float16).double()
+        assert torch.equal(torch.isinf(out), torch.isinf(want))
+        out, want = torch.where(torch.isinf(out), 0, out), torch.where(torch.isinf(want), 0, want)
+    held = kind == "bf16" and queries > 32
+    check(out, want, mass * (2.2 if held else 1), peak * (1.4 if held else 1), TYPES[kind], hd)
