@@ -56,6 +56,11 @@ struct Raw {
             for (int i = 0; i < 8; ++i) p[i] = e[i];
         }
     }
+    __device__ __forceinline__ void clamp() {  // fp32: to fp16's largest (below -65504 is code 0 either way)
+        float* e = reinterpret_cast<float*>(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = fminf(e[i], 65504.f);
+    }
     __device__ __forceinline__ float get(int i) const { return to_f32<T>(reinterpret_cast<const T*>(v)[i]); }
     __device__ __forceinline__ void set2(int i, float x, float y) {  // elements i (even) and i + 1
         if constexpr (std::is_same<T, float>::value) {
@@ -230,6 +235,15 @@ __global__ void __launch_bounds__(32 * STORE_WARPS) kv4_append_kernel(const Kv4P
                 hi = max_nan(hi, __shfl_xor_sync(FULL, hi, o));
             }
             const bool nan = lo != lo;
+            // The values are clamped as their range is.  Of 16-bit values that changes no code: b is
+            // their minimum exactly, so 65504 has code 15 already.  Of fp32 ones within 500 of 65504, b
+            // can be 16 off, more than a step.
+            if constexpr (sizeof(T) == 4) {
+                if (hi > 65504.f) {
+                    raw[i][0].clamp();
+                    raw[i][1].clamp();
+                }
+            }
             lo = fminf(fmaxf(lo, -65504.f), 65504.f);
             hi = fminf(fmaxf(hi, -65504.f), 65504.f);
             const __half sh = __float2half_rn(fifteenth(hi, lo));

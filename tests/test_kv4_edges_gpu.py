@@ -72,3 +72,23 @@ def test_largest_code_past_fp16(queries, kind, which):
         out, want = torch.where(torch.isinf(out), 0, out), torch.where(torch.isinf(want), 0, want)
     held = kind == "bf16" and queries > 32
     check(out, want, mass * (2.2 if held else 1), peak * (1.4 if held else 1), TYPES[kind], hd)
+
+
+def test_groups_that_reach_past_the_largest_value():
+    """fp32 groups near +-65504 with values beyond: clamped before they are coded."""
+    g = torch.Generator(device="cuda").manual_seed(50)
+    hd, n = 64, 400
+    lo = 65504 - 2.0 ** (torch.rand(n, 1, 1, generator=g, device="cuda") * 16 - 4)
+    x = lo + (66000 - lo) * torch.rand(n, 1, hd, generator=g, device="cuda")
+    x[:, :, 0] = lo[:, :, 0]
+    x[::4, :, 5] = 1e6
+    x[1::4, :, 5] = math.inf
+    x[2::8] = -x[2::8]
+    x[0, 0, :], x[0, 0, 1:3] = 65400, torch.tensor([65300.0, 1e6])
+    x[1, 0, :], x[1, 0, 1:3] = 65500, torch.tensor([65490.0, 70000])
+    slots = torch.randperm(n, generator=g, device="cuda")
+    for order in (torch.arange(n, device="cuda"), slots):  # whole tiles, and token by token
+        pool = mb.kv4_pool(n // 16, 1, hd, 16)
+        mb.kv4_append(pool, x, -x, order)
+        k, v = mb.kv4_read(pool, order, hd)
+        assert torch.equal(k, ref.quantize(x)[3].float()) and torch.equal(v, ref.quantize(-x)[3].float())
