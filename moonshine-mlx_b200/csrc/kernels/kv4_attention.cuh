@@ -564,7 +564,9 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2 * NC; ++e) {
-                    s[u][nt][e] = ex2(fmaf(s[u][nt][e], f[nt][e % NC], -mf[nt][e % NC]));
+                    const float x = s[u][nt][e];
+                    s[u][nt][e] = ex2(fmaf(x, f[nt][e % NC], -mf[nt][e % NC]));
+                    if (!PLAIN && x == -INFINITY) s[u][nt][e] = 0.f;  // not seen, even by a query that is NaN
                     l[nt][e % NC] += s[u][nt][e];
                 }
 #pragma unroll

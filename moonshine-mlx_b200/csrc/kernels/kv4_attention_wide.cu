@@ -676,7 +676,12 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
 #pragma unroll
                 for (int j = 16 * c; j < 16 * c + 16; ++j) {
                     const float2 x = fma2(s2[j], f2, neg2);
-                    s2[j] = make_float2(ex2(x.x), ex2(x.y));
+                    float2 p = make_float2(ex2(x.x), ex2(x.y));
+                    if constexpr (!PLAIN) {  // not seen, even by a query that is NaN
+                        if (s2[j].x == -INFINITY) p.x = 0.f;
+                        if (s2[j].y == -INFINITY) p.y = 0.f;
+                    }
+                    s2[j] = p;
                     l2 = add2(l2, s2[j]);
                 }
                 if constexpr (ROUND) {

@@ -92,3 +92,21 @@ def test_groups_that_reach_past_the_largest_value():
         mb.kv4_append(pool, x, -x, order)
         k, v = mb.kv4_read(pool, order, hd)
         assert torch.equal(k, ref.quantize(x)[3].float()) and torch.equal(v, ref.quantize(-x)[3].float())
+
+
+# ---------------------------------------------------------------- NaN
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("lens,queries,per", [(3, 5, 1), (3, 5, 3), (20, 75, 1), (1, 130, 2)])
+def test_a_query_that_is_nan_and_sees_nothing(lens, queries, per, kind):
+    """Zeros, whatever the query holds; one that sees something is NaN, the others as without it."""
+    g = torch.Generator(device="cuda").manual_seed(queries)
+    hd, blind = 64, queries - lens
+    pool, table, keys, values = build([lens], 2, hd, 16, g)
+    q = torch.randn(queries, 2 * per, hd, generator=g, device="cuda").to(TYPES[kind])
+    clean = mb.kv4_attention(q, pool, table, ints([lens]), cu_q=ints([0, queries]), max_q=queries)
+    q[0, 0, 3], q[blind - 1, 1, 2] = math.nan, math.inf
+    q[-1, 0, 7] = -math.inf
+    out = mb.kv4_attention(q, pool, table, ints([lens]), cu_q=ints([0, queries]), max_q=queries)
+    assert not out[:blind].any() and torch.isnan(out[-1, 0]).all()
+    out[-1, 0] = clean[-1, 0]
+    assert torch.equal(out, clean)
