@@ -96,6 +96,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The probability of what a query does not see: a zero that no exponential gives
+constexpr float NOT_SEEN = -0.f;
+__device__ __forceinline__ bool not_seen(float p) { return __float_as_uint(p) == 0x80000000u; }
 __device__ __forceinline__ float pow2(int n) { return __int_as_float((n + 127) << 23); }  // -126 <= n <= 127
 __device__ __forceinline__ float2 half2_of(uint32_t m) {
     return __half22float2(*reinterpret_cast<const __half2*>(&m));
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
                 for (int e = 0; e < 2 * NC; ++e) {
                     const float x = s[u][nt][e];
                     s[u][nt][e] = ex2(fmaf(x, f[nt][e % NC], -mf[nt][e % NC]));
-                    if (!PLAIN && x == -INFINITY) s[u][nt][e] = 0.f;  // not seen, even by a query that is NaN
+                    if (!PLAIN && x == -INFINITY) s[u][nt][e] = NOT_SEEN;  // even by a query that is NaN
                     l[nt][e % NC] += s[u][nt][e];
                 }
 #pragma unroll
@@ -590,8 +593,9 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 #pragma unroll
                     for (int e = 0; e < 2 * NC; ++e) {
                         const float p = s[u][nt][e], sv = e < NC ? s0 : s1, bv = e < NC ? b0 : b1;
-                        // what a query does not see adds nothing, whatever its page holds
-                        const bool none = !PLAIN && p == 0.f;
+                        // what a query does not see adds nothing, whatever its page holds; what it sees
+                        // does, a NaN even where p underflowed
+                        const bool none = !PLAIN && not_seen(p);
                         w[2 * (e / NC) + e % NC] = none ? 0.f : p * sv;
                         ob[n][nt][e % NC] = none ? ob[n][nt][e % NC] : fmaf(p, bv, ob[n][nt][e % NC]);
                     }

@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
                 }
             }
             if constexpr (!PLAIN) {
-                const int pos = first - first % KV4_TILE + i * WIDE_STEP;
+                const int pos = tile0 * KV4_TILE + i * WIDE_STEP;
 #pragma unroll
                 for (int j = 0; j < WIDE_STEP; ++j)
                     if (!((ok >> (j / KV4_TILE)) & 1) || pos + j >= lim) s[j] = -INFINITY;
@@ -677,9 +677,9 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
                 for (int j = 16 * c; j < 16 * c + 16; ++j) {
                     const float2 x = fma2(s2[j], f2, neg2);
                     float2 p = make_float2(ex2(x.x), ex2(x.y));
-                    if constexpr (!PLAIN) {  // not seen, even by a query that is NaN
-                        if (s2[j].x == -INFINITY) p.x = 0.f;
-                        if (s2[j].y == -INFINITY) p.y = 0.f;
+                    if constexpr (!PLAIN) {  // even by a query that is NaN
+                        if (s2[j].x == -INFINITY) p.x = ROUND ? 0.f : NOT_SEEN;
+                        if (s2[j].y == -INFINITY) p.y = ROUND ? 0.f : NOT_SEEN;
                     }
                     s2[j] = p;
                     l2 = add2(l2, s2[j]);
@@ -706,9 +706,9 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
                                     ob2[n] = fma2(p, bv, ob2[n]);
                                 } else {
                                     // what a query does not see adds nothing, whatever its page holds
-                                    if (p.x == 0.f) w.x = 0.f;
+                                    if (not_seen(p.x)) w.x = 0.f;
                                     else ob2[n].x = fmaf(p.x, bv.x, ob2[n].x);
-                                    if (p.y == 0.f) w.y = 0.f;
+                                    if (not_seen(p.y)) w.y = 0.f;
                                     else ob2[n].y = fmaf(p.y, bv.y, ob2[n].y);
                                 }
                                 hi[k + o] = pack_half2(w.x, w.y);
@@ -721,32 +721,29 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
                     }
                 }
             }
-            if constexpr (ROUND && !PLAIN) {
-                // what lies where V is not finite went into the product as zeros
-#pragma unroll 1
-                for (int u = 0; u < 2 * WIDE_TILES; ++u)
-                    if (const uint32_t odd = s_odd[i & 7][u])
-#pragma unroll
-                        for (int j = 0; j < WIDE_STEP; ++j)
-                            if (j / KV4_TILE + j % KV4_TILE / 8 * WIDE_TILES == u && s[j] != 0.f)
-#pragma unroll
-                                for (int n = 0; n < NG; ++n)
-                                    if ((odd >> (8 * n + j % 8)) & 1) ob2[n].x = NAN;
-            }
             tmem_st_wait();
         };
-        const int whole = (min(all_see, last) - (first - first % KV4_TILE)) / WIDE_STEP;  // stages that all rows see
+        const int whole = (min(all_see, last) - tile0 * KV4_TILE) / WIDE_STEP;  // stages that all rows see
         for (int i = 0; i < steps && good; ++i) {
             good = wait_on(&s_s[i & 3], (i >> 2) & 1, failed);
             if (!good) break;
             fence_after();
             const uint32_t ok = s_ok[i & 7];
-            bool plain = i < whole && ok == (1u << WIDE_TILES) - 1;
             if constexpr (ROUND) {
                 const uint4 x = *reinterpret_cast<const uint4*>(s_odd[i & 7]), y = *reinterpret_cast<const uint4*>(s_odd[i & 7] + 4);
-                plain = plain && !(x.x | x.y | x.z | x.w | y.x | y.y | y.z | y.w);
+                if (x.x | x.y | x.z | x.w | y.x | y.y | y.z | y.w) {
+                    // where V is not finite zeros go into the product; who sees it has a NaN
+#pragma unroll 1
+                    for (int u = 0; u < 2 * WIDE_TILES; ++u)
+#pragma unroll 1
+                        for (uint32_t odd = s_odd[i & 7][u]; odd; odd &= odd - 1) {
+                            const int bit = __ffs(odd) - 1;
+                            if (tile0 * KV4_TILE + i * WIDE_STEP + u % WIDE_TILES * KV4_TILE + u / WIDE_TILES * 8 + (bit & 7) < lim)
+                                (bit < 8 ? ob2[0] : ob2[NG - 1]).x = NAN;
+                        }
+                }
             }
-            if (plain) step(std::true_type{}, i, ok);
+            if (i < whole && ok == (1u << WIDE_TILES) - 1) step(std::true_type{}, i, ok);
             else step(std::false_type{}, i, ok);
             fence_before();
             __syncwarp();

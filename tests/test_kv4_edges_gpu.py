@@ -110,3 +110,33 @@ def test_a_query_that_is_nan_and_sees_nothing(lens, queries, per, kind):
     assert not out[:blind].any() and torch.isnan(out[-1, 0]).all()
     out[-1, 0] = clean[-1, 0]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("queries", [1, 6, 100])
+@pytest.mark.parametrize("at", [40, 99])
+@pytest.mark.parametrize("gap", [False, True])
+def test_a_nan_value_reaches_all_that_see_it(gap, at, queries, kind):
+    """By visibility, not by the size of its probability: every other position's underflows here.
+    In a whole tile and in the last, part-filled one; beside a missing page and not."""
+    g = torch.Generator(device="cuda").manual_seed(at)
+    hd, n = 96, 100
+    k, v = random_kv(n, 1, hd, torch.float32, g)
+    k[5] = 3 * torch.sign(torch.randn(1, hd, generator=g, device="cuda"))
+    v[at, 0, 70] = math.nan
+    pool = mb.kv4_pool(7, 1, hd, 16)
+    slots = torch.arange(n, device="cuda")
+    mb.kv4_append(pool, k, v, slots)
+    table = torch.arange(7, dtype=torch.int32, device="cuda")[None]
+    if gap:
+        table[0, 4] = -1
+    q = (k[5:6].expand(queries, 1, hd) * 40).to(TYPES[kind])
+    ks = mb.kv4_read(pool, slots, hd)[0].double()
+    scores = (ks[:, 0] @ q[0, 0].double()) * hd ** -0.5
+    rest = torch.cat([scores[:5], scores[6:]])
+    assert scores[5] - rest.max() > 300  # exp(-300) is 0 in fp32
+    out = mb.kv4_attention(q, pool, table, ints([n]), cu_q=ints([0, queries]), max_q=queries, causal=False)
+    assert torch.isnan(out[:, :, 64:]).all() and not torch.isnan(out[:, :, :64]).any()
+    # nobody sees it: as if it were not there
+    one = mb.kv4_attention(q, pool, table, ints([at]), cu_q=ints([0, queries]), max_q=queries, causal=False)
+    assert not torch.isnan(one).any()
