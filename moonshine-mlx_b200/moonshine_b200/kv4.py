@@ -10,7 +10,8 @@ Every call enqueues on the current stream of its tensors' device and returns wit
 so all of them can be captured into a CUDA graph, which replays with the lengths, tables and
 pages that the device memory then holds.  All tensors of a call are on one CUDA device.  A
 slice of a larger buffer can be the pool (one layer of [pages, layers, kv_heads, bytes]) as
-long as its strides are multiples of 16 bytes.  No call has a gradient.
+long as its strides are multiples of 16 bytes.  No call has a gradient: outside of
+torch.no_grad() tensors that require one are refused.
 """
 from __future__ import annotations
 
@@ -119,6 +120,11 @@ def _tokens(t, name, dtype, device, shape):
         raise ValueError(f"{name}'s last dimension must be contiguous")
 
 
+def _no_gradient(a, t, name):
+    if t.requires_grad and a.torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient and this call has none: detach it, or call under torch.no_grad()")
+
+
 def _pages(a, pool, head_dim):
     if head_dim not in a.each:
         raise ValueError(f"head_dim must be a multiple of 8 from 8 to 128, not {head_dim}")
@@ -205,6 +211,9 @@ def kv4_append(pool, k, v, slots) -> None:
     code = a.codes.get(k.dtype)
     device = pool.get_device()
     shape, ks, vs, ps = k.shape, k.stride(), v.stride(), pool.shape
+    if k.requires_grad or v.requires_grad:
+        _no_gradient(a, k, "k")
+        _no_gradient(a, v, "v")
     if not (code is not None and device >= 0 and len(shape) == 3 and len(ps) == 3 and shape[2] in a.each
             and shape[1] == ps[1] and v.shape == shape and v.dtype is k.dtype and ks[2] == vs[2] == 1
             and k.get_device() == v.get_device() == slots.get_device() == device and pool.dtype is a.u8
@@ -273,6 +282,9 @@ def kv4_attention(q, pool, block_table, lens, cu_q=None, max_q: Optional[int] = 
         raise ValueError("cu_q needs max_q, the most tokens of a row")
     if out is None:
         out = a.torch.empty(shape, dtype=q.dtype, device=q.device)
+    if q.requires_grad or out.requires_grad:
+        _no_gradient(a, q, "q")
+        _no_gradient(a, out, "out")
     os = out.stride()
     if not (code is not None and device >= 0 and len(shape) == 3 and len(ps) == 3 and len(ts) == 2
             and shape[2] in a.each and shape[1] > 0 and ps[1] > 0 and shape[1] % ps[1] == 0 and qs[2] == os[2] == 1

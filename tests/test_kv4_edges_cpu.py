@@ -42,3 +42,23 @@ for page_size in (2 ** 30 + 16, 2 ** 31 - 16):
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True,
                        timeout=60)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_tensors_that_want_a_gradient():
+    """The operators have none: a call that would cut the graph is refused, one under no_grad is not
+    (it goes on to the next check, which CPU tensors fail)."""
+    pool, slots = torch.zeros(4, 2, 16 * 72, dtype=torch.uint8), torch.zeros(3, dtype=torch.int64)
+    table, lens = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    x, y = torch.zeros(3, 2, 64), torch.zeros(3, 2, 64, requires_grad=True)
+    for k, v, name in ((y, x, "k"), (x, y, "v"), (y * 2, x, "k")):
+        with pytest.raises(ValueError, match=name + " requires a gradient"):
+            mb.kv4_append(pool, k, v, slots)
+    for q, out, name in ((y, None, "q"), (x, y, "out")):
+        with pytest.raises(ValueError, match=name + " requires a gradient"):
+            mb.kv4_attention(q, pool, table, lens, out=out)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        mb.kv4_append(pool, y, y, slots)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        mb.kv4_attention(y, pool, table, lens, out=y)
+    with pytest.raises(ValueError, match="CUDA"):
+        mb.kv4_attention(y.detach(), pool, table, lens)
