@@ -6,16 +6,21 @@
 // so the matrix instructions take the codes themselves, and the scales multiply the fp32 scores
 // and the probabilities.
 //
-// Scores are integer products: the codes as bytes (3 operations per word of 8) times q as fixed
-// point of 16 bits (24 for fp32) in planes of bytes, sums exact (fp32 starts them at
-// -8 sum(q), so that they are those of d and s d q and b sum(q) do not cancel).  For V a nibble
-// becomes fp16 by one AND-OR into the mantissa of 1024 (the odd nibbles in place, as 16 c) and one
-// packed multiply-add, 9 operations per word, after a byte permute, since its fragments want two
-// positions side by side.  Probabilities times scales are rounded to fp16, as one value for bf16
-// results (which keep 8 bits), as two otherwise.  (fp16
-// codes for both cost 6 operations more per word of K; codes taken as the fp16 subnormals that
-// masked nibbles already are cost fewer, but the tensor core aligns its sums by the exponent
-// field, which lost 6 to 10 bits, and sums of one-sided codes as much again.)
+// For V, and for the scores of 16-bit queries, a nibble becomes fp16 by one AND-OR into the
+// mantissa of 1024 (the odd nibbles in place, as 16 c) and one packed multiply-add, 9 operations
+// per word; V's come after a byte permute, since its fragments want two positions side by side.
+// (Codes taken as the fp16 subnormals that masked nibbles already are cost fewer, but the
+// tensor core aligns its sums by the exponent field, which lost 6 to 10 bits, and sums of one-sided
+// codes as much again.)  Such queries are fp16 after a power of two, exact down to 2^-28 of a
+// row's largest: as 16-bit fixed point, which makes integer products of 3 operations per word and
+// 4 to 6 us less of the 54 and 96 below, one large channel took the bits of all others (1000 times
+// the rest, their scores were off by a hundredth).
+// Scores of fp32 queries are integer products: the codes as bytes times q as fixed point of
+// 24 bits in planes of bytes (16 for the decoder step with bf16 weights, whose queries are sums
+// of bf16 products), sums exact (with 24 bits they start at -8 sum(q), so that they are those of
+// d and s d q and b sum(q) do not cancel).
+// Probabilities times scales are rounded to fp16, as one value for bf16 results (which keep 8
+// bits), as two otherwise.
 //
 // S^T = K q^T and O^T = V^T P^T: positions and dims are the 16 rows of the products, queries
 // their 8 columns, since one K/V head rarely has more query rows in a decode step; the score
@@ -26,8 +31,8 @@
 //
 // Bound: issue inside a run (60 to 80 % of the slots), and 4 to 6 us of latency per CTA around
 // them (2560 CTAs of one position take 16 us).  bf16, at the cache's bytes: 256 contexts of 187 ..
-// 1500 on 10 heads of 64, 50 us (3.2 TB/s, half of copy bandwidth); four of 16K .. 131K on 32 heads
-// of 128, 4 per K/V head, 86 to 89 us (4.3 TB/s, 66 %); one of 1500 in fp32, 10 us.
+// 1500 on 10 heads of 64, 54 us (3.0 TB/s, 46 % of copy bandwidth); four of 16K .. 131K on 32 heads
+// of 128, 4 per K/V head, 96 us (3.9 TB/s, 61 %); one of 1500 in fp32, 10 us.
 #pragma once
 
 #include <climits>
@@ -82,6 +87,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 
 template <class T> constexpr bool is_step = std::is_same<T, Step>::value || std::is_same<T, StepSplit>::value;
 template <class T> constexpr bool is_f32 = std::is_same<T, float>::value || std::is_same<T, StepSplit>::value;
+template <class T> constexpr bool is_int = is_f32<T> || is_step<T>;  // scores as integer products: fp32 queries
 template <class T> constexpr bool is_bf16 = std::is_same<T, __nv_bfloat16>::value || std::is_same<T, Step>::value;
 
 // element `at` of the result
@@ -219,7 +225,7 @@ __device__ __forceinline__ int over(int n, int d) { return d == 1 ? n : n / d; }
 template <class T, int NG, int NT, int NC>
 struct AttShape {
     static constexpr int ROWS = 4 * NC * NT;
-    static constexpr int QP = is_f32<T> ? 3 : 2;                               // byte planes of q
+    static constexpr int QP = is_f32<T> ? 3 : 2;                               // planes of q: bytes, or halves of each word's dims
     static constexpr int PP = is_bf16<T> ? 1 : 2;                              // fp16 planes of the probabilities
     static constexpr int SU = NG == 2 ? 2 : 4;                                 // tiles per ring stage
     static constexpr int QROW = 64 * NG + 8;                                   // bytes per q row, padded
@@ -236,7 +242,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
                                                                        const AttSplit sp, int ring_bytes) {
     using S = AttShape<T, NG, NT, NC>;
     constexpr int ROWS = S::ROWS, QP = S::QP, PP = S::PP, SU = S::SU;
-    constexpr bool F32 = is_f32<T>;
+    constexpr bool F32 = is_f32<T>, INT = is_int<T>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t s_bar[ATT_WARPS][ATT_STAGES];
     __shared__ uint32_t s_ok[ATT_WARPS][ATT_STAGES];
@@ -320,9 +326,10 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         for (int i = 0; i < ATT_STAGES; ++i)
             if (wid + i * W < runs) copy(look(tile0, tiles, wid + i * W), i);
 
-    // q as fixed point relative to its row's largest, 16 or 24 bits, in planes of signed bytes in
-    // fragment order (dims 0 2 4 6, 1 3 5 7 of a word); a negative scale goes into q.  A q that
-    // is not finite makes its row NaN by its factor.
+    // q in fragment order; a negative scale goes into it.  16-bit types: fp16 after a power of two, in
+    // planes of a word's dims 0 4 1 5 and 2 6 3 7.  fp32: fixed point relative to its row's largest,
+    // 16 or 24 bits, in planes of signed bytes (dims 0 2 4 6, 1 3 5 7).  A q that is not finite
+    // makes its row NaN by its factor.
     int8_t* qb = reinterpret_cast<int8_t*>(smem + ring_bytes);
     constexpr int MAGIC = 0x4b400000;  // 1.5 2^23 as bits: sums onto it read as floats, exact below 2^22
     for (int r = wid; r < ROWS; r += W) {
@@ -355,6 +362,31 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         }
         mx = warp_max(mx);
         odd = __any_sync(FULL, odd);
+        if constexpr (!INT) {
+            // the exponent of the row's largest; rows below 2^-100 keep less
+            const int e2 = mx > 0.f && !odd ? min(100, max(-100, (__float_as_int(mx) >> 23) - 127)) : 0;
+            const float up = a.scale < 0.f ? -pow2(14 - e2) : pow2(14 - e2);
+            float sum[NG];
+#pragma unroll
+            for (int n = 0; n < NG; ++n) sum[n] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2 * NG; ++k) {
+                const int d = lane + 32 * k, i = d & 7, pl = (i >> 1) & 1, at = (d & ~7) + 4 * (i & 1) + 2 * (i >> 2);
+                const __half v = __float2half_rn(odd ? 0.f : x[k] * up);
+                *reinterpret_cast<__half*>(qb + (pl * ROWS + r) * S::QROW + at) = v;
+                sum[k >> 1] += __half2float(v);
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                sum[n] = warp_sum(sum[n]);
+                if (lane == 0) s_qs[r][n] = sum[n];
+            }
+            if (lane == 0) {
+                s_f[r] = odd ? NAN : fmaxf(fabsf(a.scale) * LOG2E * pow2(e2 - 14), 1e-37f);
+                s_end[r] = row.end(a, qi);
+            }
+            continue;
+        }
         // the largest integer whose bytes are all signed ones, less what rounding may add
         constexpr float top = QP == 2 ? 32600.f : 8355000.f;
         const float up = mx > 1e-30f && !odd ? (a.scale < 0.f ? -top : top) / mx : 0.f;
@@ -465,12 +497,27 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
             const uint32_t tile = st + u * tile_bytes;
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
-                int acc[QP][NT][4];
+                [[maybe_unused]] int acc[QP][NT][4];
+                [[maybe_unused]] float dots[NT][4];
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
                     const int j = 2 * n + jj;
                     // lanes past the vector's last word read what lies behind; their q is zero
                     const uint2 w = lds64(tile + k_at[j]);
+                    if constexpr (!INT) {
+                        uint32_t x[4], y[4];
+                        codes_minus_8(w.x, x);
+                        codes_minus_8(w.y, y);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int pl = 0; pl < QP; ++pl) {
+                                const uint32_t* b = qf[pl][nt][j];
+                                if (jj == 0 && pl == 0) mma16816_new(dots[nt], x[0], y[0], x[1], y[1], b[0], b[1]);
+                                else mma16816(dots[nt], x[2 * pl], y[2 * pl], x[2 * pl + 1], y[2 * pl + 1], b[0], b[1]);
+                            }
+                        continue;
+                    }
                     const uint32_t x0 = w.x & 0x0f0f0f0fu, x1 = (w.x >> 4) & 0x0f0f0f0fu;
                     const uint32_t y0 = w.y & 0x0f0f0f0fu, y1 = (w.y >> 4) & 0x0f0f0f0fu;
 #pragma unroll
@@ -489,16 +536,20 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 k = half2_of(i ? meta.y : meta.x);
-                    const float kb = F32 ? fmaf(8.f, k.x, k.y) : k.y;
+                    const float kb = F32 || !INT ? fmaf(8.f, k.x, k.y) : k.y;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < NC; ++c) {
                             float dot = 0.f;
+                            if constexpr (INT) {
 #pragma unroll
-                            for (int pl = QP - 1; pl >= 0; --pl) {
-                                const float part = __int_as_float(acc[pl][nt][2 * i + c]) - 12582912.f;
-                                dot = pl == QP - 1 ? part : fmaf(dot, 256.f, part);
+                                for (int pl = QP - 1; pl >= 0; --pl) {
+                                    const float part = __int_as_float(acc[pl][nt][2 * i + c]) - 12582912.f;
+                                    dot = pl == QP - 1 ? part : fmaf(dot, 256.f, part);
+                                }
+                            } else {
+                                dot = dots[nt][2 * i + c];
                             }
                             float& d = s[u][nt][NC * i + c];
                             d = fmaf(kb, qs[n][nt][c], n == 0 ? dot * k.x : fmaf(dot, k.x, d));

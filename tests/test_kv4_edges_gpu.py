@@ -140,3 +140,47 @@ def test_a_nan_value_reaches_all_that_see_it(gap, at, queries, kind):
     # nobody sees it: as if it were not there
     one = mb.kv4_attention(q, pool, table, ints([at]), cu_q=ints([0, queries]), max_q=queries, causal=False)
     assert not torch.isnan(one).any()
+
+
+# ---------------------------------------------------------------- queries of unlike sizes
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("queries", [1, 4, 16, 100])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_one_large_query_channel(hd, queries, kind):
+    """One channel of q 1000 times the others, its keys the same at all positions (the group's
+    minimum, -4, so code 0 and exactly b): it moves no probability, the small channels decide.
+    Two positions, so the result is the mean of two values under a difference of scores.
+
+    A score is exact but for fp32 sums: of a group the codes' sum (4 products of 16 dims on the
+    tensor cores, each cut by 2^-23 of its largest term), and 3 operations of 2^-24 that join it
+    with the bias, 11 in units of 2^-24 of the terms, and one more that adds the second group; terms
+    are below 15 s and 2 |b| times |q| each.  bf16 with many queries takes keys rounded by 2^-12
+    (those of the large channel are exact).  Two scores' errors move the result by at most a
+    quarter of the values' difference each, so by |score error| times the largest value."""
+    g = torch.Generator(device="cuda").manual_seed(hd + queries)
+    n, heads = 2, 3
+    k = (torch.randn(n, 1, hd, generator=g, device="cuda") * 1.5).clamp(-3.9, 3.9)
+    k[:, :, 0] = -4.0
+    k[:, :, 64:65] = -4.0
+    v = torch.randn(n, 1, hd, generator=g, device="cuda")
+    pool = mb.kv4_pool(1, 1, hd, 16)
+    slots = torch.arange(n, device="cuda")
+    mb.kv4_append(pool, k, v, slots)
+    ks, vs = (x.double() for x in mb.kv4_read(pool, slots, hd))
+    assert (ks[:, 0, 0] == -4).all()
+    q = torch.randn(queries, heads, hd, generator=g, device="cuda")
+    q[:, :, 0] = 1000.0
+    q = q.to(TYPES[kind])
+    table = ints([[0]])
+    out = mb.kv4_attention(q, pool, table, ints([n]), cu_q=ints([0, queries]), max_q=queries, causal=False)
+    want, _, peak = ref.attention(q, [ks], [vs], [n], [0, queries], False, hd ** -0.5)
+    size, groups = q.double().abs(), -(-hd // 64)
+    terms = (size.sum(-1) * (8 + 2 * 4)) * hd ** -0.5  # 15 s is at most 8
+    score = terms * (11 + groups) * 2.0 ** -24
+    if kind == "bf16" and queries * heads > 32:
+        score = score + size[:, :, 1:].sum(-1) * 4 * 2.0 ** -12 * hd ** -0.5
+    plane = 2.0 ** -12 + 2.0 ** -13 if kind == "bf16" else 2.0 ** -22
+    half = torch.finfo(TYPES[kind]).eps / 2
+    tol = want.abs() * half + (peak * (score + 2 * plane + 2.0 ** -20)).unsqueeze(-1)
+    off = (out.double() - want).abs() - tol
+    assert off.max().item() <= 0, off.max().item()
