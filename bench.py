@@ -236,7 +236,7 @@ def _events(torch, stream):
     return a, b
 
 
-def leg_batched(mb, synth, root, torch, barrier, rank, local, reps=3):
+def leg_batched(mb, synth, root, torch, barrier, rank, local, reps=3, cross_kv_bits=0):
     """ms_generate_batch on small bf16: 64 utterances of U(5, 15) s, 128 forced tokens each,
     host buffers in and out; CUDA events on the model's stream around the public call."""
     import numpy as np
@@ -247,7 +247,7 @@ def leg_batched(mb, synth, root, torch, barrier, rank, local, reps=3):
     brng = np.random.Generator(np.random.PCG64(7))
     blens = (brng.uniform(5, 15, size=64) * 16000).astype(int) // 80 * 80
     baudio = [synth.synth_audio(int(n), 100 + i) for i, n in enumerate(blens)]
-    bm = mb.MoonshineModel.load(bpath, device=local)
+    bm = mb.MoonshineModel.load(bpath, device=local, cross_kv_bits=cross_kv_bits)
     s = torch.cuda.ExternalStream(bm.cuda_stream)
     bm.generate_batch(baudio, forced_len=128)
     b_enc, b_dec, b_ms = [], [], []
@@ -274,7 +274,7 @@ def leg_batched(mb, synth, root, torch, barrier, rank, local, reps=3):
                       f"(median of {reps})"}
 
 
-def leg_sharded(mb, synth, root, torch, dist, barrier, rank, world, local, reps=2, sub_batch=256):
+def leg_sharded(mb, synth, root, torch, dist, barrier, rank, world, local, reps=2, sub_batch=256, cross_kv_bits=0):
     """A fixed job of 256 medium bf16 utterances of U(2, 30) s, each decoding its own limit
     ceil(6.5 s) with EOS ignored, partitioned by length over the ranks (shard.py).  Each rank
     runs its share through ms_generate_batch in length-sorted groups of at most `sub_batch`
@@ -293,18 +293,20 @@ def leg_sharded(mb, synth, root, torch, dist, barrier, rank, world, local, reps=
     order = sorted(share, key=lambda i: -int(lens[i]))
     groups = [order[k:k + sub_batch] for k in range(0, len(order), sub_batch)]
     audio = {i: synth.synth_audio(int(lens[i]), 1000 + i) for i in share}
-    m = mb.MoonshineModel.load(path, device=local)
+    m = mb.MoonshineModel.load(path, device=local, cross_kv_bits=cross_kv_bits)
     s = torch.cuda.ExternalStream(m.cuda_stream)
     m.generate_batch([audio[i] for i in groups[0]], forced_len=-1)   # warm-up: weights, graphs
-    times, results = [], {}
+    times, results, dec_ms = [], {}, 0.0
     for rep in range(reps):
         barrier()
         torch.cuda.synchronize()
         e0, e1 = _events(torch, s)
         torch.cuda.nvtx.range_push(f"sharded_{rep}")  # one timed job's kernels, for ncu --nvtx
         e0.record(s)
+        dec_ms = 0.0
         for g in groups:
-            ids, _ = m.generate_batch([audio[i] for i in g], forced_len=-1)
+            ids, st = m.generate_batch([audio[i] for i in g], forced_len=-1)
+            dec_ms += st.decode_ms
             for i, r in zip(g, ids):
                 results[i] = r
         e1.record(s)
@@ -331,7 +333,7 @@ def leg_sharded(mb, synth, root, torch, dist, barrier, rank, world, local, reps=
     return {"workload": "medium bf16 weights, 256 utterances of U(2, 30) s (a fixed job, partitioned by length "
                         "over the GPUs), each decoding ceil(6.5 tokens per second) with EOS ignored",
             "n_gpus": world, "tokens": tok_all, "audio_s": round(audio_s, 1),
-            "job_s": round(t_max, 4), "tokens_per_s": round(tok_all / t_max, 1),
+            "job_s": round(t_max, 4), "decode_ms": round(dec_ms, 1), "tokens_per_s": round(tok_all / t_max, 1),
             "rtfx": round(audio_s / t_max, 1), "rank_imbalance": round(t_max / t_mean, 4),
             "utterances_per_gpu_call": min(sub_batch, len(share)),
             "timing": "CUDA events on each rank's model stream around its generate_batch calls (host buffers, "
@@ -434,6 +436,8 @@ def main():
     ap.add_argument("--no-batched", action="store_true", help="skip the small-model batched leg")
     ap.add_argument("--no-sharded", action="store_true", help="skip the medium-model sharded job")
     ap.add_argument("--no-streaming", action="store_true", help="skip the 512-stream leg")
+    ap.add_argument("--cross-kv-bits", type=int, default=0, choices=[0, 4],
+                    help="cross-attention K/V of the batched and sharded legs (4: in 4-bit pages)")
     ap.add_argument("--stream-chunks", type=int, default=125, help="80 ms chunks per stream")
     ap.add_argument("--seconds", type=float, default=30.0, help="audio length (profiling cases)")
     ap.add_argument("--tokens", type=int, default=200, help="forced decode length (profiling cases)")
@@ -597,9 +601,11 @@ def main():
         qm.close()
         barrier()
 
-    bleg = None if args.no_batched else leg_batched(mb, synth, root, torch, barrier, rank, local)
+    bleg = None if args.no_batched else leg_batched(mb, synth, root, torch, barrier, rank, local,
+                                                     cross_kv_bits=args.cross_kv_bits)
     barrier()
-    sleg = None if args.no_sharded else leg_sharded(mb, synth, root, torch, dist, barrier, rank, world, local)
+    sleg = None if args.no_sharded else leg_sharded(mb, synth, root, torch, dist, barrier, rank, world, local,
+                                                     cross_kv_bits=args.cross_kv_bits)
     barrier()
     stleg = None
     if not args.no_streaming:
@@ -650,6 +656,8 @@ def main():
             line["batched"] = bleg
         if sleg is not None:
             line["sharded"] = sleg
+        if args.cross_kv_bits:
+            line["cross_kv_bits"] = args.cross_kv_bits
         if stleg is not None:
             line["streaming"] = stleg
         if world == 1 and not args.no_cpu_baseline:
