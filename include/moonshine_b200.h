@@ -473,10 +473,11 @@ ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* tokens, int3
  * nothing; tokens of no row are left as they are.  A NaN reaches every query that sees its
  * position, however small the probability, and no other.  A row's table spans at most 2^30
  * positions; max_q * heads is below 2^30, and below 2^24 per K/V head.  Softmax and sums are fp32;
- * the products take the codes exactly, q exactly down to 2^-28 of each (token, head)'s largest value
- * (MS_F32: as fixed point of 24 bits relative to it; below 1e-30 it counts as zero), and the
- * probabilities as one fp16 value (MS_BF16) or two.  With more than 32 query rows per K/V head
- * MS_BF16 takes keys and values rounded to fp16 (held to +-65504). */
+ * the products take the codes exactly, q as fixed point of 24 bits relative to each (token, head)'s
+ * largest value (below 1e-30 it counts as zero; 16-bit q with more than 4 query rows per K/V head:
+ * exactly, down to 2^-28 of it), and the probabilities as one fp16 value (MS_BF16) or two.  With
+ * more than 32 query rows per K/V head MS_BF16 takes keys and values rounded to fp16 (held to
+ * +-65504). */
 typedef struct {
     const void* q;                                /* [q_tokens][heads][head_dim] */
     void* out;                                    /* the same shape; may not overlap q */

@@ -6,21 +6,22 @@
 // so the matrix instructions take the codes themselves, and the scales multiply the fp32 scores
 // and the probabilities.
 //
-// For V, and for the scores of 16-bit queries, a nibble becomes fp16 by one AND-OR into the
-// mantissa of 1024 (the odd nibbles in place, as 16 c) and one packed multiply-add, 9 operations
-// per word; V's come after a byte permute, since its fragments want two positions side by side.
-// (Codes taken as the fp16 subnormals that masked nibbles already are cost fewer, but the
-// tensor core aligns its sums by the exponent field, which lost 6 to 10 bits, and sums of one-sided
-// codes as much again.)  Such queries are fp16 after a power of two, exact down to 2^-28 of a
-// row's largest: as 16-bit fixed point, which makes integer products of 3 operations per word and
-// 4 to 6 us less of the 54 and 96 below, one large channel took the bits of all others (1000 times
-// the rest, their scores were off by a hundredth).
-// Scores of fp32 queries are integer products: the codes as bytes times q as fixed point of
-// 24 bits in planes of bytes (16 for the decoder step with bf16 weights, whose queries are sums
-// of bf16 products), sums exact (with 24 bits they start at -8 sum(q), so that they are those of
-// d and s d q and b sum(q) do not cancel).
-// Probabilities times scales are rounded to fp16, as one value for bf16 results (which keep 8
-// bits), as two otherwise.
+// V's nibbles become fp16 by one AND-OR into the mantissa of 1024 (the odd nibbles in place, as 16
+// c) and one packed multiply-add, 9 operations per word, after a byte permute, since its
+// fragments want two positions side by side.  (Codes taken as the fp16 subnormals that masked
+// nibbles already are cost fewer, but the tensor core aligns its sums by the exponent field, which
+// lost 6 to 10 bits, and sums of one-sided codes as much again.)  Probabilities times scales
+// are rounded to fp16, as one value for bf16 results (which keep 8 bits), as two otherwise.
+//
+// Scores of up to 4 query rows are integer products: the codes as bytes (3 operations per word)
+// times q as fixed point of 24 bits in three planes of bytes, sums exact.  Rows have two columns of
+// the products there, which take two planes at a time.  So have fp32 queries of more rows, three
+// products, and those of the decoder step with bf16 weights (sums of bf16 products) in 16 bits, two.
+// (fp32 starts the sums at -8 sum(q), so that they are those of d and s d q and b sum(q) do not
+// cancel.)  16-bit queries of more rows are fp16 after a power of two, exact down to 2^-28 of a
+// row's largest, and the codes for them made as V's; for up to 4 rows that costs 4 us more of the
+// 50 and 91 below.  16-bit fixed point is not enough: one channel 1000 times the others took
+// their bits, and scores were off by a hundredth.
 //
 // S^T = K q^T and O^T = V^T P^T: positions and dims are the 16 rows of the products, queries
 // their 8 columns, since one K/V head rarely has more query rows in a decode step; the score
@@ -31,8 +32,8 @@
 //
 // Bound: issue inside a run (60 to 80 % of the slots), and 4 to 6 us of latency per CTA around
 // them (2560 CTAs of one position take 16 us).  bf16, at the cache's bytes: 256 contexts of 187 ..
-// 1500 on 10 heads of 64, 54 us (3.0 TB/s, 46 % of copy bandwidth); four of 16K .. 131K on 32 heads
-// of 128, 4 per K/V head, 96 us (3.9 TB/s, 61 %); one of 1500 in fp32, 10 us.
+// 1500 on 10 heads of 64, 50 us (3.2 TB/s, half of copy bandwidth); four of 16K .. 131K on 32 heads
+// of 128, 4 per K/V head, 91 us (4.1 TB/s, 64 %); one of 1500 in fp32, 10 us.
 #pragma once
 
 #include <climits>
@@ -87,7 +88,6 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 
 template <class T> constexpr bool is_step = std::is_same<T, Step>::value || std::is_same<T, StepSplit>::value;
 template <class T> constexpr bool is_f32 = std::is_same<T, float>::value || std::is_same<T, StepSplit>::value;
-template <class T> constexpr bool is_int = is_f32<T> || is_step<T>;  // scores as integer products: fp32 queries
 template <class T> constexpr bool is_bf16 = std::is_same<T, __nv_bfloat16>::value || std::is_same<T, Step>::value;
 
 // element `at` of the result
@@ -221,11 +221,14 @@ __device__ __forceinline__ int splits_of(int end, int chunk) { return end <= chu
 __device__ __forceinline__ int over(int n, int d) { return d == 1 ? n : n / d; }  // d == 1 for most models' heads
 
 // Queries of one K/V head: ROWS (token, head) rows, token major, in NT n-tiles of 8 columns; with
-// NC = 1 only the even columns are used, which halves the softmax work for up to 4 rows.
+// NC = 1 (up to 4 rows) a row has two columns, for two planes of q at a time in the scores, and only
+// the even one after them, which halves the softmax work.
 template <class T, int NG, int NT, int NC>
 struct AttShape {
     static constexpr int ROWS = 4 * NC * NT;
-    static constexpr int QP = is_f32<T> ? 3 : 2;                               // planes of q: bytes, or halves of each word's dims
+    static constexpr bool INT = NC == 1 || is_f32<T> || is_step<T>;            // scores as integer products
+    static constexpr int QP = NC == 1 || is_f32<T> ? 3 : 2;                    // planes of q: bytes, or (not INT) halves of its words
+    static constexpr int QM = NC == 1 ? 2 : QP;                                // score products
     static constexpr int PP = is_bf16<T> ? 1 : 2;                              // fp16 planes of the probabilities
     static constexpr int SU = NG == 2 ? 2 : 4;                                 // tiles per ring stage
     static constexpr int QROW = 64 * NG + 8;                                   // bytes per q row, padded
@@ -241,8 +244,8 @@ template <class T, int NG, int NT, int NC, int HD>
 __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attention_kernel(const Kv4Pool pool, const Kv4Attention a,
                                                                        const AttSplit sp, int ring_bytes) {
     using S = AttShape<T, NG, NT, NC>;
-    constexpr int ROWS = S::ROWS, QP = S::QP, PP = S::PP, SU = S::SU;
-    constexpr bool F32 = is_f32<T>, INT = is_int<T>;
+    constexpr int ROWS = S::ROWS, QP = S::QP, QM = S::QM, PP = S::PP, SU = S::SU;
+    constexpr bool F32 = is_f32<T>, INT = S::INT;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t s_bar[ATT_WARPS][ATT_STAGES];
     __shared__ uint32_t s_ok[ATT_WARPS][ATT_STAGES];
@@ -326,10 +329,10 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         for (int i = 0; i < ATT_STAGES; ++i)
             if (wid + i * W < runs) copy(look(tile0, tiles, wid + i * W), i);
 
-    // q in fragment order; a negative scale goes into it.  16-bit types: fp16 after a power of two, in
-    // planes of a word's dims 0 4 1 5 and 2 6 3 7.  fp32: fixed point relative to its row's largest,
-    // 16 or 24 bits, in planes of signed bytes (dims 0 2 4 6, 1 3 5 7).  A q that is not finite
-    // makes its row NaN by its factor.
+    // q in fragment order; a negative scale goes into it.  Fixed point relative to its row's largest,
+    // 16 or 24 bits, in planes of signed bytes (dims 0 2 4 6, 1 3 5 7 of a word), or fp16 after a
+    // power of two, in planes of a word's dims 0 4 1 5 and 2 6 3 7.  A q that is not finite makes its
+    // row NaN by its factor.
     int8_t* qb = reinterpret_cast<int8_t*>(smem + ring_bytes);
     constexpr int MAGIC = 0x4b400000;  // 1.5 2^23 as bits: sums onto it read as floats, exact below 2^22
     for (int r = wid; r < ROWS; r += W) {
@@ -425,20 +428,20 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     }
     __syncthreads();
     pdl_trigger();
-    uint32_t qf[QP][NT][2 * NG][2];
+    uint32_t qf[QM][NT][2 * NG][2];
     float f[NT][NC], qs[NG][NT][NC];
     int from[NG][QP][NT][NC];  // fp32 only: MAGIC - 8 sum(q)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int pl = 0; pl < QP; ++pl)
+        for (int m = 0; m < QM; ++m)
 #pragma unroll
             for (int j = 0; j < 2 * NG; ++j) {
-                const int r = NC == 2 ? nt * 8 + g : nt * 4 + (g >> 1);
+                const int r = NC == 2 ? nt * 8 + g : nt * 4 + (g >> 1), pl = NC == 2 ? m : min(2, 2 * m + (g & 1));
                 uint2 v = *reinterpret_cast<const uint2*>(qb + (pl * ROWS + r) * S::QROW + 8 * (4 * j + t));
-                if (NC == 1 && (g & 1)) v = make_uint2(0, 0);
-                qf[pl][nt][j][0] = v.x;
-                qf[pl][nt][j][1] = v.y;
+                if (NC == 1 && m == 1 && (g & 1)) v = make_uint2(0, 0);
+                qf[m][nt][j][0] = v.x;
+                qf[m][nt][j][1] = v.y;
             }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
             const uint32_t tile = st + u * tile_bytes;
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
-                [[maybe_unused]] int acc[QP][NT][4];
+                [[maybe_unused]] int acc[QM][NT][4];
                 [[maybe_unused]] float dots[NT][4];
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
@@ -511,10 +514,10 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int pl = 0; pl < QP; ++pl) {
-                                const uint32_t* b = qf[pl][nt][j];
-                                if (jj == 0 && pl == 0) mma16816_new(dots[nt], x[0], y[0], x[1], y[1], b[0], b[1]);
-                                else mma16816(dots[nt], x[2 * pl], y[2 * pl], x[2 * pl + 1], y[2 * pl + 1], b[0], b[1]);
+                            for (int m = 0; m < QM; ++m) {
+                                const uint32_t* b = qf[m][nt][j];
+                                if (jj == 0 && m == 0) mma16816_new(dots[nt], x[0], y[0], x[1], y[1], b[0], b[1]);
+                                else mma16816(dots[nt], x[2 * m], y[2 * m], x[2 * m + 1], y[2 * m + 1], b[0], b[1]);
                             }
                         continue;
                     }
@@ -523,11 +526,12 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int pl = 0; pl < QP; ++pl) {
+                        for (int m = 0; m < QM; ++m) {
                             if (jj == 0)
-                                imma16832_on(acc[pl][nt], x0, y0, x1, y1, qf[pl][nt][j][0], qf[pl][nt][j][1],
-                                             from[n][pl][nt][0], from[n][pl][nt][NC - 1]);
-                            else imma16832(acc[pl][nt], x0, y0, x1, y1, qf[pl][nt][j][0], qf[pl][nt][j][1]);
+                                imma16832_on(acc[m][nt], x0, y0, x1, y1, qf[m][nt][j][0], qf[m][nt][j][1],
+                                             from[n][NC == 1 ? 2 * m : m][nt][0],
+                                             NC == 2 ? from[n][m][nt][NC - 1] : m == 0 ? from[n][1][nt][0] : MAGIC);
+                            else imma16832(acc[m][nt], x0, y0, x1, y1, qf[m][nt][j][0], qf[m][nt][j][1]);
                         }
                 }
                 const uint4 meta = lds128(tile + m_at + 128 * n);
@@ -545,7 +549,8 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
                             if constexpr (INT) {
 #pragma unroll
                                 for (int pl = QP - 1; pl >= 0; --pl) {
-                                    const float part = __int_as_float(acc[pl][nt][2 * i + c]) - 12582912.f;
+                                    const int sum = NC == 2 ? acc[pl][nt][2 * i + c] : acc[pl >> 1][nt][2 * i + (pl & 1)];
+                                    const float part = __int_as_float(sum) - 12582912.f;
                                     dot = pl == QP - 1 ? part : fmaf(dot, 256.f, part);
                                 }
                             } else {
