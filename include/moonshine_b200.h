@@ -471,7 +471,7 @@ ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* tokens, int3
  * lens[b] - n + i (lens counts the queries' own positions); otherwise all.  Query head h reads
  * K/V head h / (heads / kv_heads).  out = softmax(scale q k^T) v, zeros for a query that sees
  * nothing; tokens of no row are left as they are.  A NaN reaches every query that sees its
- * position, however small the probability, and no other.  A row's table spans at most 2^30
+ * position, however small the probability, and no other; a score past 2e38 is one.  A row's table spans at most 2^30
  * positions; max_q * heads is below 2^30, and below 2^24 per K/V head.  Softmax and sums are fp32;
  * the products take the codes exactly, q as fixed point of 24 bits relative to each (token, head)'s
  * largest value (below 1e-30 it counts as zero; 16-bit q with more than 4 query rows per K/V head:

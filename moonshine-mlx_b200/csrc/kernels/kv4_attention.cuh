@@ -154,6 +154,31 @@ __device__ __forceinline__ void mma16816_new(float (&c)[4], uint32_t a0, uint32_
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+// two fp32 operations in one
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 // maximum and sum over the eight lanes that hold one column pair
 __device__ __forceinline__ float rows_max(float v) {
 #pragma unroll
@@ -367,7 +392,7 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         odd = __any_sync(FULL, odd);
         if constexpr (!INT) {
             // the exponent of the row's largest; rows below 2^-100 keep less
-            const int e2 = mx > 0.f && !odd ? min(100, max(-100, (__float_as_int(mx) >> 23) - 127)) : 0;
+            const int e2 = mx > 0.f && !odd ? max(-100, (__float_as_int(mx) >> 23) - 127) : 0;
             const float up = a.scale < 0.f ? -pow2(14 - e2) : pow2(14 - e2);
             float sum[NG];
 #pragma unroll
@@ -457,14 +482,16 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
     }
 
     // per lane: columns 2 t (and 2 t + 1), c = 0 (1); accumulator element c + 2 i is row g + 8 i.
-    // Scores are kept without the factor f: m is the running maximum of those, mf = m f.
-    float o[NG][4][NT][4], ob[NG][NT][NC], m[NT][NC], mf[NT][NC], l[NT][NC];
+    // Scores are kept without the factor f: m is the running maximum of those, and probabilities are
+    // 2^((score - m) f), since score f - m f would be off by the rounding of m f, which is no longer small
+    // where scores pass 2^24.
+    float o[NG][4][NT][4], ob[NG][NT][NC], m[NT][NC], l[NT][NC];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             m[nt][c] = -INFINITY;
-            mf[nt][c] = l[nt][c] = 0.f;
+            l[nt][c] = 0.f;
 #pragma unroll
             for (int n = 0; n < NG; ++n) ob[n][nt][c] = 0.f;
         }
@@ -600,10 +627,8 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const float mx = fmaxf(m[nt][c], rows_max(top[nt][c]));
-                    const float now = mx == -INFINITY ? 0.f : mx * f[nt][c];
-                    const float corr = m[nt][c] == -INFINITY ? 0.f : ex2(mf[nt][c] - now), both = corr * down;
+                    const float corr = m[nt][c] == -INFINITY ? 0.f : ex2((m[nt][c] - mx) * f[nt][c]), both = corr * down;
                     m[nt][c] = mx;
-                    mf[nt][c] = now;
                     l[nt][c] *= corr;
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
@@ -622,11 +647,17 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2 * NC; ++e) {
-                    const float x = s[u][nt][e];
-                    s[u][nt][e] = ex2(fmaf(x, f[nt][e % NC], -mf[nt][e % NC]));
-                    if (!PLAIN && x == -INFINITY) s[u][nt][e] = NOT_SEEN;  // even by a query that is NaN
-                    l[nt][e % NC] += s[u][nt][e];
+                for (int e = 0; e < 2 * NC; e += 2) {
+                    const float2 x = make_float2(s[u][nt][e], s[u][nt][e + 1]);
+                    const float2 y = mul2(add2(x, make_float2(-m[nt][0], -m[nt][NC - 1])), make_float2(f[nt][0], f[nt][NC - 1]));
+                    s[u][nt][e] = ex2(y.x);
+                    s[u][nt][e + 1] = ex2(y.y);
+                    if constexpr (!PLAIN) {  // even by a query that is NaN
+                        if (x.x == -INFINITY) s[u][nt][e] = NOT_SEEN;
+                        if (x.y == -INFINITY) s[u][nt][e + 1] = NOT_SEEN;
+                    }
+                    l[nt][0] += s[u][nt][e];
+                    l[nt][NC - 1] += s[u][nt][e + 1];
                 }
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
@@ -736,8 +767,9 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
                             make_float2(fmaf(o[n][mt][nt][c], up, bias), fmaf(o[n][mt][nt][2 + c], up, bias));
             }
             if (g == 0) {
-                s_m[wid][r] = m[nt][c] == -INFINITY ? -INFINITY : mf[nt][c];
-                s_l[wid][r] = lr;
+                const float mf = m[nt][c] == -INFINITY ? -INFINITY : m[nt][c] * f[nt][c];
+                s_m[wid][r] = mf;
+                s_l[wid][r] = m[nt][c] > -INFINITY && fabsf(mf) == INFINITY ? NAN : lr;  // a score past fp32's range
             }
         }
     if (W > 1) __syncthreads();

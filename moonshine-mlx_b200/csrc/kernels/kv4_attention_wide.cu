@@ -130,32 +130,6 @@ __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st
 __device__ __forceinline__ void sts128(uint32_t a, const uint32_t* v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
-// two fp32 operations in one
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\t"
-        "mov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\t"
-        "mov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-
 // an (s, b) word with an infinity or a NaN
 __device__ __forceinline__ bool not_finite(uint32_t w) {
     return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
@@ -552,7 +526,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
             const float mx = max_nan(to_f32<T>(top[0].x), to_f32<T>(top[0].y));
             const bool odd = !(mx < INFINITY);
             // its exponent; rows below 2^-100 keep less
-            const int e2 = mx > 0.f && !odd ? min(100, max(-100, (__float_as_int(mx) >> 23) - 127)) : 0;
+            const int e2 = mx > 0.f && !odd ? max(-100, (__float_as_int(mx) >> 23) - 127) : 0;
             const float up = odd ? 0.f : a.scale < 0.f ? -pow2(14 - e2) : pow2(14 - e2);
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
@@ -585,7 +559,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
         const int qi = mine ? over_near(row0 + r, per, each_per) : 0, h = mine ? kvh * per + (row0 + r - qi * per) : 0;
         const long long tok = row.q0 + (long long)qi;
         const int lim = mine ? min(last, row.end(a, qi)) : last;
-        float ref = -INFINITY;  // log2 reference: p = 2^(score f - ref)
+        float ref = -INFINITY, add = 0.f;  // p = 2^((score - ref) f + add)
         float2 l2 = make_float2(0.f, 0.f), ob2[NG];
 #pragma unroll
         for (int n = 0; n < NG; ++n) ob2[n] = make_float2(0.f, 0.f);
@@ -641,16 +615,17 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
             const float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
                                     fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
             // the reference moves when p (s) could pass 2^15; it is set so that they are below 2^7
-            float most = top * f;
+            float lift = 0.f;
             if constexpr (!ROUND) {
                 const float4 a = four(s_vmax[i & 1]), b = four(s_vmax[i & 1] + 4);
-                most += __log2f(fmaxf(fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))),
-                                      5.9604645e-8f));
+                lift = __log2f(fmaxf(fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))),
+                                     5.9604645e-8f));
             }
-            const bool move = most > ref + 15.f;  // also from -inf; never for -inf or NaN scores
+            const bool move = fmaf(top - ref, f, add) + lift > 15.f;  // also from -inf; never for -inf or NaN scores
             if (__any_sync(FULL, move)) {
-                const float to = move ? most - 7.f : ref;
-                const float corr = !move || ref == -INFINITY ? (move ? 0.f : 1.f) : ex2(ref - to);
+                const float to = move ? top : ref, gain = move ? 7.f - lift : add;
+                const float corr = !move ? 1.f : ref == -INFINITY ? 0.f : ex2(fmaf(ref - to, f, gain - add));
+                add = gain;
                 ref = to;
                 l2 = mul2(l2, make_float2(corr, corr));
 #pragma unroll
@@ -669,13 +644,12 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
                     }
                 }
             }
-            const float neg = ref == -INFINITY ? 0.f : -ref;
-            const float2 neg2 = make_float2(neg, neg);
+            const float2 neg2 = make_float2(-ref, -ref), add2f = make_float2(add, add);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
                 for (int j = 16 * c; j < 16 * c + 16; ++j) {
-                    const float2 x = fma2(s2[j], f2, neg2);
+                    const float2 x = fma2(add2(s2[j], neg2), f2, add2f);
                     float2 p = make_float2(ex2(x.x), ex2(x.y));
                     if constexpr (!PLAIN) {  // even by a query that is NaN
                         if (s2[j].x == -INFINITY) p.x = ROUND ? 0.f : NOT_SEEN;
@@ -751,7 +725,9 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
         }
         if (steps > 0 && good) good = wait_on(&s_pv[(steps - 1) & 3], ((steps - 1) >> 2) & 1, failed);
         fence_after();
-        const float l = good ? l2.x + l2.y : NAN;
+        const float log2_ref = ref == -INFINITY ? -INFINITY : fmaf(ref, f, -add);
+        const bool past = ref > -INFINITY && fabsf(log2_ref) == INFINITY;  // a score past fp32's range
+        const float l = good && !past ? l2.x + l2.y : NAN;
         const float inv = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
         const bool done = n_split == 1;
         const long long each = a.q_tokens * a.heads, at = part_nr * each + tok * a.heads + h;
@@ -790,7 +766,7 @@ __global__ void __launch_bounds__(WideSmem<NG, is_bf16<T>>::THREADS, 2) kv4_atte
                 }
             }
         }
-        if (mine && !done) reinterpret_cast<float2*>(sp.part + sp.splits * each * hd)[at] = make_float2(ref, l);
+        if (mine && !done) reinterpret_cast<float2*>(sp.part + sp.splits * each * hd)[at] = make_float2(log2_ref, l);
         }
     }
     fence_before();

@@ -184,3 +184,32 @@ def test_one_large_query_channel(hd, queries, kind):
     tol = want.abs() * half + (peak * (score + 2 * plane + 2.0 ** -20)).unsqueeze(-1)
     off = (out.double() - want).abs() - tol
     assert off.max().item() <= 0, off.max().item()
+
+
+# ---------------------------------------------------------------- the end of fp32's range
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("queries", [1, 6, 100])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_at_the_end_of_fp32(sign, queries, kind):
+    """Queries of 1e35, whose scores fit: the position with the largest one alone, its value but for the
+    roundings of one probability (2^-12 + 2^-13 in bf16, 2^-22 in fp32).  Queries of 3e38, whose scores do
+    not: NaN, as a sum of infinities is, and not the zeros of a query that sees nothing."""
+    g = torch.Generator(device="cuda").manual_seed(60)
+    hd, n = 64, 40
+    k = 1 + torch.rand(n, 1, hd, generator=g, device="cuda")
+    v = torch.randn(n, 1, hd, generator=g, device="cuda")
+    pool = mb.kv4_pool(3, 1, hd, 16)
+    slots = torch.arange(n, device="cuda")
+    mb.kv4_append(pool, k, v, slots)
+    ks, vs = (x.double() for x in mb.kv4_read(pool, slots, hd))
+    table = ints([[0, 1, 2]])
+    for size, fits in ((1e35, True), (3e38, False)):
+        q = torch.full((queries, 1, hd), sign * size, device="cuda").to(TYPES[kind])
+        out = mb.kv4_attention(q, pool, table, ints([n]), cu_q=ints([0, queries]), max_q=queries, causal=False)
+        if fits:
+            want = vs[(ks[:, 0].sum(-1) * sign).argmax()].expand(queries, 1, hd)
+            plane = 2.0 ** -12 + 2.0 ** -13 if kind == "bf16" else 2.0 ** -22
+            tol = want.abs() * torch.finfo(TYPES[kind]).eps / 2 + vs.abs().max() * (2 * plane + 2.0 ** -20)
+            assert ((out.double() - want).abs() <= tol).all()
+        else:
+            assert torch.isnan(out).all()
