@@ -10,10 +10,10 @@ namespace {
 int rows_per_cta(const Kv4Attention& a, int kv_heads, int head_dim) {
     // A stage of the wide kernel takes as long for 20 rows as for 128.  Against the other, us for
     // ragged requests of 4 K/V heads, (33 of 1000 .. 8000 positions; 64 of 190 .. 1500):
-    //   bf16, heads of 64   20 rows (75; 36) and (64; 37), 32 (79; 36) and (75; 39), 64 (87; 40) and (121; 68)
-    //   bf16, heads of 128  20 rows (117; 53) and (100; 52), 32 (121; 54) and (111; 57), 35 (109; 57) and (132; 74)
-    //   fp16, heads of 64   32 rows (95; 49) and (76; 43), 48 (107; 53) and (103; 57), 64 (116; 54) and (132; 72)
-    //   fp16, heads of 128  48 rows (217; 100) and (161; 75), 64 (253; 105) and (213; 103)
+    //   bf16, heads of 64   20 rows (81; 38) and (67; 37), 32 (73; 39) and (67; 38), 35 (81; 43) and (90; 52)
+    //   bf16, heads of 128  20 rows (113; 53) and (99; 50), 32 (116; 55) and (110; 55), 35 (112; 56) and (135; 67)
+    //   fp16, heads of 64   35 rows (114; 53) and (105; 51), 48 (107; 54) and (105; 55), 64 (118; 55) and (144; 69)
+    //   fp16, heads of 128  48 rows (200; 101) and (150; 80), 64 (226; 104) and (200; 99)
     // (fp16 takes the codes exactly, so its softmax does more.  fp32 has no wide kernel: its
     // products need more planes.)
     const long long rows = (long long)a.max_q * (a.heads / kv_heads);

@@ -3,7 +3,7 @@
 //
 // bf16 results (ROUND): K and V enter the products as fp16(s c + b), three bits more than the
 // results keep, one rounding each.  Then S = Q K^T and O += P V are plain products and the softmax
-// thread has 3.5 operations per position, where the exact form has 9.
+// thread has 4 operations per position, where the exact form has 9.
 // fp16 results: the products take the codes d = c - 8 themselves, S_n = Q_n D_n^T for each group n
 // of 64 dims, scores sum_n s_tn S_n + (b_tn + 8 s_tn) sum(q_n), and P_n = p_t s_tn (two fp16
 // planes); sum p_t (b_tn + 8 s_tn) stays in the thread.
@@ -23,10 +23,10 @@
 // thread) a few times per CTA.
 //
 // Two CTAs share an SM.  Bound: latency inside the roles; of a stage's 1300 cycles (64 dims, bf16)
-// the 64 exponentials of a warp are 512, and the tensor pipe is active 14 % of the time.  Measured,
-// 592 CTAs of 2048 positions: bf16 103 us (64 dims), 156 us (128); fp16 155 and 288 us.  8 prompts of
-// up to 512 tokens over up to 4096 positions, 16 heads on 4: 83 us, of which the longest rows' CTAs,
-// which meet on some SMs, take all: cut into pieces of 2048 the parts cost more (90 to 98 us).
+// the 64 exponentials of a warp are 512, and the tensor pipe is active 16 % of the time.  Measured,
+// 592 CTAs of 2048 positions: bf16 116 us (64 dims), 166 us (128); fp16 170 and 292 us.  8 prompts of
+// up to 512 tokens over up to 4096 positions, 16 heads on 4: 86 us, of which the longest rows' CTAs,
+// which meet on some SMs, take all: cut into pieces of 2048 the parts cost more (7 to 15 us).
 #define KV4_ATTENTION_KERNELS
 #include "kv4_attention.cuh"
 
