@@ -387,7 +387,7 @@ cudaError_t launch_gather_cross(const float* const* src32, const void* const* sr
 
 // ---------------------------------------------------------------- 4-bit paged K/V cache
 // KV4_STEP: fp32 queries and the bf16 planes of a GEMM input as the result (the batched decoder
-// step's); products as for bf16, or as for fp32 when lo_off asks for the low plane.
+// step's); probabilities as for bf16, or as for fp32 when lo_off asks for the low plane.
 enum Kv4Type { KV4_F32 = 0, KV4_F16 = 1, KV4_BF16 = 2, KV4_STEP = 3 };
 // Pages of 4-bit keys and values (layout: kv4.cuh); strides in bytes, multiples of 16.
 struct Kv4Pool {

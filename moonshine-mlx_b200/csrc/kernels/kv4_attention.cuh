@@ -15,10 +15,9 @@
 //
 // Scores of up to 4 query rows are integer products: the codes as bytes (3 operations per word)
 // times q as fixed point of 24 bits in three planes of bytes, sums exact.  Rows have two columns of
-// the products there, which take two planes at a time.  So have fp32 queries of more rows, three
-// products, and those of the decoder step with bf16 weights (sums of bf16 products) in 16 bits, two.
-// (fp32 starts the sums at -8 sum(q), so that they are those of d and s d q and b sum(q) do not
-// cancel.)  16-bit queries of more rows are fp16 after a power of two, exact down to 2^-28 of a
+// the products there, which take two planes at a time; fp32 queries of more rows are three
+// products.  (fp32 results start the sums at -8 sum(q), so that they are those of d and s d q and
+// b sum(q) do not cancel.)  16-bit queries of more rows are fp16 after a power of two, exact down to 2^-28 of a
 // row's largest, and the codes for them made as V's; for up to 4 rows that costs 4 us more of the
 // 50 and 91 below.  16-bit fixed point is not enough: one channel 1000 times the others took
 // their bits, and scores were off by a hundredth.
@@ -72,8 +71,8 @@ constexpr int ATT_STAGES = 2;   // ring slots per warp
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Element types of the batched decoder step: fp32 queries, bf16 planes of a GEMM input out
-struct Step { float v; };       // products as for bf16
-struct StepSplit { float v; };  // products as for fp32, and the low plane
+struct Step { float v; };       // probabilities as for bf16
+struct StepSplit { float v; };  // probabilities as for fp32, and the low plane
 
 template <class T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<Step>(Step v) { return v.v; }
@@ -252,7 +251,7 @@ template <class T, int NG, int NT, int NC>
 struct AttShape {
     static constexpr int ROWS = 4 * NC * NT;
     static constexpr bool INT = NC == 1 || is_f32<T> || is_step<T>;            // scores as integer products
-    static constexpr int QP = NC == 1 || is_f32<T> ? 3 : 2;                    // planes of q: bytes, or (not INT) halves of its words
+    static constexpr int QP = INT ? 3 : 2;                                     // planes of q: bytes, or halves of its words
     static constexpr int QM = NC == 1 ? 2 : QP;                                // score products
     static constexpr int PP = is_bf16<T> ? 1 : 2;                              // fp16 planes of the probabilities
     static constexpr int SU = NG == 2 ? 2 : 4;                                 // tiles per ring stage
@@ -354,9 +353,9 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
         for (int i = 0; i < ATT_STAGES; ++i)
             if (wid + i * W < runs) copy(look(tile0, tiles, wid + i * W), i);
 
-    // q in fragment order; a negative scale goes into it.  Fixed point relative to its row's largest,
-    // 16 or 24 bits, in planes of signed bytes (dims 0 2 4 6, 1 3 5 7 of a word), or fp16 after a
-    // power of two, in planes of a word's dims 0 4 1 5 and 2 6 3 7.  A q that is not finite makes its
+    // q in fragment order; a negative scale goes into it.  Fixed point of 24 bits relative to its row's
+    // largest, in planes of signed bytes (dims 0 2 4 6, 1 3 5 7 of a word), or fp16 after a power of
+    // two, in planes of a word's dims 0 4 1 5 and 2 6 3 7.  A q that is not finite makes its
     // row NaN by its factor.
     int8_t* qb = reinterpret_cast<int8_t*>(smem + ring_bytes);
     constexpr int MAGIC = 0x4b400000;  // 1.5 2^23 as bits: sums onto it read as floats, exact below 2^22
@@ -415,8 +414,8 @@ __global__ void __launch_bounds__(NT == 1 ? 32 * ATT_WARPS : 128, 2) kv4_attenti
             }
             continue;
         }
-        // the largest integer whose bytes are all signed ones, less what rounding may add
-        constexpr float top = QP == 2 ? 32600.f : 8355000.f;
+        // the largest integer of three signed bytes, less what rounding may add
+        constexpr float top = 8355000.f;
         const float up = mx > 1e-30f && !odd ? (a.scale < 0.f ? -top : top) / mx : 0.f;
         int sum[NG][QP];
 #pragma unroll

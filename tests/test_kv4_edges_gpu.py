@@ -8,7 +8,7 @@ torch = pytest.importorskip("torch")
 
 import kv4_reference as ref  # noqa: E402
 import moonshine_b200 as mb  # noqa: E402
-from test_kv4_gpu import TYPES, build, check, ints, random_kv  # noqa: E402
+from test_kv4_gpu import TYPES, build, check, ints, random_kv, tolerance  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +213,50 @@ def test_scores_at_the_end_of_fp32(sign, queries, kind):
             assert ((out.double() - want).abs() <= tol).all()
         else:
             assert torch.isnan(out).all()
+
+
+# ---------------------------------------------------------------- the batched decoder step's form
+@pytest.fixture(scope="module")
+def step_attention(tmp_path_factory):
+    import ctypes as C
+    import os
+    import subprocess
+    so = str(tmp_path_factory.mktemp("kv4_step") / "kv4_step.so")
+    here, package = os.path.dirname(os.path.abspath(__file__)), os.path.dirname(os.path.abspath(mb.__file__))
+    mb._L()
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I/usr/local/cuda/include",
+                    "-I" + os.path.join(os.path.dirname(package), "csrc", "kernels"), os.path.join(here, "kv4_step.cpp"),
+                    os.path.join(package, "libmoonshine_b200.so"), "-Wl,-rpath," + package, "-o", so], check=True)
+    f, P, I = C.CDLL(so).step_attention, C.c_void_p, C.c_int
+    f.restype, f.argtypes = C.c_int64, [P, I, I, I, I, P, P, I, I, P, I, P, C.c_float, C.c_int64, P, P, P]
+    return f
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("lens,kv_heads,per,hd", [([40, 0, 7], 8, 1, 40), ([375, 64], 10, 1, 64), ([100, 33, 1], 2, 3, 40),
+                                                  ([129, 750, 20], 2, 5, 64), ([300], 1, 8, 56), ([9000, 80], 2, 8, 64)])
+def test_decoder_step(lens, kv_heads, per, hd, split, step_attention):
+    """fp32 queries, one channel of each 300 times the others; the result in bf16, or as the sum of two
+    bf16 planes, which keep 2^-17 of it."""
+    g = torch.Generator(device="cuda").manual_seed(sum(lens) + per)
+    page, heads, rows = 64, kv_heads * per, len(lens)
+    pool, table, keys, values = build(lens, kv_heads, hd, page, g)
+    q = torch.randn(rows, heads, hd, generator=g, device="cuda")
+    q[:, :, 5] *= 300
+    n = rows * heads * hd
+    out = torch.full((2, rows, heads, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+    status, length = torch.zeros(1, dtype=torch.int32, device="cuda"), ints(lens)
+    args = (pool.data_ptr(), pool.shape[0], kv_heads, hd, page, q.data_ptr(), out.data_ptr(), heads, rows, table.data_ptr(),
+            table.shape[1], length.data_ptr(), hd ** -0.5, n if split else 0)
+    work = torch.empty(max(step_attention(*args, None, None, None), 16), dtype=torch.uint8, device="cuda")
+    assert step_attention(*args, work.data_ptr(), status.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    want, mass, peak = ref.attention(q, keys, values, lens, list(range(rows + 1)), False, hd ** -0.5)
+    got = out[0].double() + (out[1].double() if split else 0)
+    # fp32's roundings before the result and its planes' 2^-17, or bf16's
+    if split:
+        off = (got - want).abs() - tolerance(want, mass, peak, torch.float32, hd) - want.abs() * 2.0 ** -17
+        assert off.max().item() <= 0, off.max().item()
+    else:
+        check(got, want, mass, peak, torch.bfloat16, hd)
+        assert (out[1] == 7.0).all()
+    assert status.item() == 0
