@@ -403,9 +403,8 @@ ms_status ms_generate_long(ms_model* model, const float* audio, int64_t n_sample
  * and pages that the device memory then holds.  Argument errors are found before anything
  * is enqueued.
  *
- * Pages.  A pool holds `pages` pages of page_size positions (a multiple of 16, at most
- * 2^30), each position
- * with kv_heads K and V vectors of head_dim values (a multiple of 8, at most 128).  A vector's
+ * Pages.  A pool holds `pages` pages of page_size positions (a multiple of 16, at most 2^30), each
+ * position with kv_heads K and V vectors of head_dim values (a multiple of 8, at most 128).  A vector's
  * values are cut into groups of 64 (the last one shorter); a group is stored as 4-bit codes c,
  * an fp16 scale s and an fp16 bias b (the affine form of the quantized checkpoints) and
  * stands for s c + b: b = fp16(min), s = fp16(fp32((max - min) / 15)), c = how many of the
@@ -471,13 +470,13 @@ ms_status ms_kv4_read(const ms_kv4_pool* pool, const ms_kv4_tokens* tokens, int3
  * lens[b] - n + i (lens counts the queries' own positions); otherwise all.  Query head h reads
  * K/V head h / (heads / kv_heads).  out = softmax(scale q k^T) v, zeros for a query that sees
  * nothing; tokens of no row are left as they are.  A NaN reaches every query that sees its
- * position, however small the probability, and no other; a score past 2e38 is one.  A row's table spans at most 2^30
- * positions; max_q * heads is below 2^30, and below 2^24 per K/V head.  Softmax and sums are fp32;
- * the products take the codes exactly, q as fixed point of 24 bits relative to each (token, head)'s
- * largest value (below 1e-30 it counts as zero; 16-bit q with more than 4 query rows per K/V head:
- * exactly, down to 2^-28 of it), and the probabilities as one fp16 value (MS_BF16) or two.  With
- * more than 32 query rows per K/V head MS_BF16 takes keys and values rounded to fp16 (held to
- * +-65504). */
+ * position, however small the probability, and no other; a score past 2e38 makes its query's row
+ * NaN.  A row's table spans at most 2^30 positions; max_q * heads is below 2^30, and below 2^24
+ * per K/V head.  Softmax and sums are fp32; the products take the codes exactly, q as fixed point of
+ * 24 bits relative to each (token, head)'s largest value (below 1e-30 it counts as zero; 16-bit q
+ * with more than 4 query rows per K/V head: exactly, down to 2^-28 of it), and the probabilities
+ * as one fp16 value (MS_BF16) or two.  With more than 32 query rows per K/V head MS_BF16 takes keys
+ * and values rounded to fp16 (held to +-65504). */
 typedef struct {
     const void* q;                                /* [q_tokens][heads][head_dim] */
     void* out;                                    /* the same shape; may not overlap q */
